@@ -1,0 +1,54 @@
+"""What of the 8-bit operators needs no GPU: the checks of weights and rows, how a product is cut."""
+import pytest
+import torch
+
+from tiny_llm_infer_b200 import ops
+from tiny_llm_infer_b200.ops import fp8
+
+
+def e4m3(*shape):
+    return torch.zeros(shape, dtype=torch.float8_e4m3fn)
+
+
+def test_weights_say_what_they_want():
+    ops.Fp8Weight(e4m3(200, 144), torch.ones(2, 2))
+    ops.Fp8Weight(e4m3(272, 128), torch.ones(4, 1), gated=True)
+    for q, scales, gated in ((e4m3(200, 144), torch.ones(2, 1), False), (e4m3(200, 144), torch.ones(1, 2), False), (e4m3(272, 128), torch.ones(3, 1), True),
+                             (e4m3(264, 128), torch.ones(4, 1), True), (e4m3(16, 24), torch.ones(1, 1), False), (e4m3(0, 16), torch.ones(0, 1), False),
+                             (torch.zeros(16, 16), torch.ones(1, 1), False), (e4m3(16, 16), torch.ones(1, 1, dtype=torch.float64), False),
+                             (e4m3(32, 32).t()[:16], torch.ones(1, 1), False)):
+        with pytest.raises(ops.KernelError):
+            ops.Fp8Weight(q, scales, gated)
+
+
+def test_rows_say_what_they_want():
+    assert tuple(ops.Fp8Rows(e4m3(3, 144), torch.ones(3, 2)).shape) == (3, 144)
+    for q, scales in ((e4m3(3, 144), torch.ones(3, 1)), (e4m3(3, 144), torch.ones(2, 2)), (e4m3(3, 24), torch.ones(3, 1)), (torch.zeros(3, 16), torch.ones(3, 1))):
+        with pytest.raises(ops.KernelError):
+            ops.Fp8Rows(q, scales)
+
+
+def test_values_follow_the_layout_of_the_scales():
+    q = torch.ones(272, 144).to(torch.float8_e4m3fn)
+    plain = ops.Fp8Weight(q, torch.arange(6.0).view(3, 2)).values()
+    assert plain[127, 127] == 0 and plain[127, 128] == 1 and plain[128, 0] == 2 and plain[271, 143] == 5
+    gated = ops.Fp8Weight(q, torch.arange(8.0).view(4, 2), gated=True).values()
+    # row 16 j + i is gate row 8 j + i, eight further its up row; gate row 128 is row 256
+    assert gated[0, 0] == 0 and gated[8, 0] == 2 and gated[247, 0] == 0 and gated[255, 143] == 3 and gated[256, 0] == 4 and gated[264, 0] == 6
+
+
+@pytest.mark.parametrize("rows", [33, 64, 128, 129, 500, 2048, 100000])
+@pytest.mark.parametrize("n,k", [(8, 16), (1024, 128), (4096, 4096), (24576, 4096), (130, 12288)])
+def test_shares_cover_all_blocks_and_none_is_empty(rows, n, k):
+    columns, splits, each = fp8._plan(rows, n, k, 148)
+    kb = -(-k // 128)
+    assert columns in (128, 256) and (splits - 1) * each < kb <= splits * each
+
+
+def test_tensors_of_the_host_are_refused():
+    with pytest.raises(ops.KernelError):
+        ops.quantize_rows_fp8(torch.zeros(2, 16))
+    with pytest.raises(ops.KernelError):
+        ops.quantize_weight_fp8(torch.zeros(16, 16))
+    with pytest.raises(ops.KernelError):
+        ops.linear(torch.zeros(2, 16), ops.Fp8Weight(e4m3(16, 16), torch.ones(1, 1)))

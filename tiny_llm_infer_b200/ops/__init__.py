@@ -22,6 +22,9 @@ from typing import Optional
 import torch
 
 from ..csrc import build as _build
+from . import fp8 as _fp8
+from .fp8 import (Fp8Rows, Fp8Weight, add_rmsnorm_fp8, linear_fp8, linear_swiglu_fp8, quantize_rows_fp8,  # noqa: F401
+                  quantize_weight_fp8)
 
 F32, BF16 = 0, 1
 _DT = {torch.float32: F32, torch.bfloat16: BF16}
@@ -139,6 +142,7 @@ def _declare(h) -> None:
         fn = getattr(h, name)
         fn.argtypes = args
         fn.restype = i32
+    _fp8.declare(h)
     h.tllm_delta_rule_lanes.argtypes = [i32]
     h.tllm_delta_rule_lanes.restype = i32
     h.tllm_delta_rule_state_floats.argtypes = [i32, i32, i32, i32, i32]
@@ -715,7 +719,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torch.dtyp
            bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y[T, N] = x[T, K] . weight[N, K]^T with float32 accumulation.  A weight kept in
     float32 is multiplied in float32 whatever the activations are stored in.  ``bias`` [N] (the weight's type) is
-    added in the library product's epilogue."""
+    added in the library product's epilogue.  An ``Fp8Weight`` is multiplied by ``linear_fp8``, which also takes ``Fp8Rows``."""
+    if isinstance(weight, Fp8Weight):
+        if bias is not None:
+            raise KernelError("a product with an 8-bit weight takes no bias")
+        return linear_fp8(x, weight, out_dtype)
     if not x.is_cuda:
         raise KernelError("linear takes CUDA tensors")
     want = out_dtype or x.dtype
@@ -755,12 +763,18 @@ def gemm_skinny_swiglu(x: torch.Tensor, w_gate_up: torch.Tensor, act: str = "sil
     return out
 
 
-def linear_swiglu(x: torch.Tensor, w_gate_up: torch.Tensor, out_dtype: torch.dtype,
+def linear_swiglu(x: torch.Tensor, w_gate_up: torch.Tensor, out_dtype: Optional[torch.dtype] = None,
                   interleaved: bool = False, act: str = "silu", consts=None) -> torch.Tensor:
     """silu(x . Wg^T) * (x . Wu^T) for w_gate_up = [Wg; Wu], or with the rows of Wg and Wu
     interleaved by eight (``interleave_gate_up``).  With enough bfloat16 rows the product and the
     activation are one tcgen05 kernel, with few rows and interleaved weights one weight-streaming
-    kernel; otherwise the product is followed by the SwiGLU kernel."""
+    kernel; otherwise the product is followed by the SwiGLU kernel.  A gated ``Fp8Weight`` gives ``Fp8Rows``
+    (``linear_swiglu_fp8``)."""
+    if isinstance(w_gate_up, Fp8Weight):
+        if out_dtype not in (None, Fp8Rows):
+            raise KernelError(f"a gated product with an 8-bit weight gives 8-bit rows, not {out_dtype}")
+        return linear_swiglu_fp8(x, w_gate_up, act, consts)
+    out_dtype = out_dtype or x.dtype
     rows, k = x.shape
     inter = w_gate_up.shape[0] // 2
     plain = x.dtype == w_gate_up.dtype == out_dtype == torch.bfloat16 and x.is_contiguous() \

@@ -1,0 +1,313 @@
+"""Weights, rows and caches in 8 bits: e4m3 values with float32 scales, and the kernels that read them (``csrc/fp8*.cu``).
+
+A block of numbers with largest magnitude A is kept as e4m3(x / s) and s = max(A, 2^-100) / 448.  A weight has a scale per
+block of 128 x 128, a row that meets it one per 128 columns, a key or value of the cache one per head.  A product sums the 128 terms of
+a block in float32, multiplies by both scales and adds the blocks in float32:
+
+    y[t, n] = sum_b sx[t, b] sw[n / 128, b] sum_{k in b} qx[t, k] qw[n, k]
+
+``ops.linear`` and ``ops.linear_swiglu`` take an ``Fp8Weight`` in the place of a weight, and rows in bfloat16, float32 or as ``Fp8Rows``.
+Which kernel runs goes by the number of rows, the last bits of a row with it; what is rounded to 8 bits does not depend on it.
+Infinities and NaN in a row of x reach the outputs of that row alone (as NaN), in a weight those of its block's columns.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+BLOCK = 128
+E4M3 = torch.float8_e4m3fn
+SMALLEST = 2.0 ** -100
+LARGEST = 448.0
+
+
+def _ops():
+    from .. import ops
+    return ops
+
+
+def declare(h) -> None:
+    """Signatures of the C entry points."""
+    vp, i32, f32, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
+    sigs = {
+        "tllm_fp8_rows": [vp, i32, vp, vp, i32, i32, vp],
+        "tllm_fp8_gated_rows": [vp, i32, vp, vp, i32, i32, i32, f32, f32, vp],
+        "tllm_add_rmsnorm_fp8": [vp, vp, i32, vp, i32, f32, vp, vp, i32, i32, vp],
+        "tllm_fp8_weight": [vp, i32, vp, vp, i32, i32, i32, vp],
+        "tllm_fp8_skinny": [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, f32, f32, vp],
+        "tllm_fp8_tcgen05": [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, f32, f32, vp, vp],
+        "tllm_fp8_join": [vp, i32, i64, vp, i32, vp],
+    }
+    for name, args in sigs.items():
+        fn = getattr(h, name)
+        fn.argtypes = args
+        fn.restype = i32
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _refuse(text: str):
+    raise _ops().KernelError(text)
+
+
+def _here(*tensors) -> None:
+    """Contiguous CUDA tensors of the current device (the kernels go to its current stream)."""
+    current = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda or not t.is_contiguous():
+            _refuse("kernels take contiguous CUDA tensors")
+        if current is None:
+            current = torch.cuda.current_device()
+        if t.device.index != current:
+            _refuse(f"a tensor of {t.device}, the current device is cuda:{current}")
+
+
+class Fp8Weight:
+    """A weight [N, K] as e4m3 values ``q`` and float32 ``scales`` [ceil(N / 128), ceil(K / 128)].  ``gated``: the rows are N / 2 gate
+    and N / 2 up rows interleaved by eight (``ops.interleave_gate_up``), and the scales [2 ceil(N / 2 / 128), ceil(K / 128)] are those
+    of 128 gate rows, of the up rows that belong to them, and so on.  K is a multiple of 16."""
+    __slots__ = ("q", "scales", "gated")
+
+    def __init__(self, q: torch.Tensor, scales: torch.Tensor, gated: bool = False):
+        if q.dtype != E4M3 or q.dim() != 2 or scales.dtype != torch.float32:
+            _refuse(f"an 8-bit weight is a matrix of float8_e4m3fn with float32 scales, got {q.dtype} {tuple(q.shape)} and {scales.dtype}")
+        n, k = q.shape
+        if n == 0 or k == 0 or k % 16:
+            _refuse(f"an 8-bit weight's columns are a multiple of 16, got {n} x {k}")
+        if gated and n % 16:
+            _refuse(f"interleaved gate and up rows come in sixteens, got {n}")
+        want = (2 * _blocks(n // 2) if gated else _blocks(n), _blocks(k))
+        if tuple(scales.shape) != want:
+            _refuse(f"an 8-bit weight of {n} x {k} has scales {list(want)}, got {list(scales.shape)}")
+        if q.device != scales.device or not q.is_contiguous() or not scales.is_contiguous() or q.data_ptr() % 16:
+            _refuse("an 8-bit weight and its scales are contiguous on one device, the weight 16-byte aligned")
+        self.q, self.scales, self.gated = q, scales, bool(gated)
+
+    @property
+    def shape(self):
+        return self.q.shape
+
+    @property
+    def dtype(self):
+        return self.q.dtype
+
+    @property
+    def device(self):
+        return self.q.device
+
+    def values(self) -> torch.Tensor:
+        """The float32 numbers that the weight stands for (for tests and comparisons)."""
+        n, k = self.q.shape
+        rows = torch.arange(n, device=self.q.device)
+        if self.gated:
+            rows = 2 * ((rows // 16 * 8) // BLOCK) + rows // 8 % 2
+        else:
+            rows = rows // BLOCK
+        columns = torch.arange(k, device=self.q.device) // BLOCK
+        return self.q.to(torch.float32) * self.scales[rows][:, columns]
+
+
+class Fp8Rows:
+    """Rows [T, K] as e4m3 values ``q`` and float32 ``scales`` [T, ceil(K / 128)]: what the products take."""
+    __slots__ = ("q", "scales")
+
+    def __init__(self, q: torch.Tensor, scales: torch.Tensor):
+        if q.dtype != E4M3 or q.dim() != 2 or scales.dtype != torch.float32 or tuple(scales.shape) != (q.shape[0], _blocks(q.shape[1])):
+            _refuse(f"8-bit rows are a matrix of float8_e4m3fn with float32 scales [rows, columns / 128], got {q.dtype} {tuple(q.shape)}, "
+                    f"{scales.dtype} {tuple(scales.shape)}")
+        if q.shape[1] == 0 or q.shape[1] % 16:
+            _refuse(f"8-bit rows have a multiple of 16 columns, got {q.shape[1]}")
+        self.q, self.scales = q, scales
+
+    @property
+    def shape(self):
+        return self.q.shape
+
+    @property
+    def dtype(self):
+        return self.q.dtype
+
+    @property
+    def device(self):
+        return self.q.device
+
+    def values(self) -> torch.Tensor:
+        columns = torch.arange(self.q.shape[1], device=self.q.device) // BLOCK
+        return self.q.to(torch.float32) * self.scales[:, columns]
+
+
+def _empty_rows(rows: int, k: int, device) -> Fp8Rows:
+    return Fp8Rows(torch.empty((rows, k), dtype=E4M3, device=device), torch.empty((rows, _blocks(k)), dtype=torch.float32, device=device))
+
+
+def _columns(k: int) -> None:
+    if k == 0 or k % 16:
+        _refuse(f"8-bit rows have a multiple of 16 columns, got {k}")
+
+
+def quantize_weight_fp8(weight: torch.Tensor, gated: bool = False) -> Fp8Weight:
+    """A bfloat16 or float32 weight [N, K] in 8 bits (K a multiple of 16); ``gated``: its rows are interleaved gate and up rows."""
+    ops = _ops()
+    _here(weight)
+    if weight.dim() != 2 or weight.numel() == 0:
+        _refuse(f"a weight is a matrix, got {tuple(weight.shape)}")
+    n, k = weight.shape
+    _columns(k)
+    if gated and n % 16:
+        _refuse(f"interleaved gate and up rows come in sixteens, got {n}")
+    q = torch.empty((n, k), dtype=E4M3, device=weight.device)
+    scales = torch.empty((2 * _blocks(n // 2) if gated else _blocks(n), _blocks(k)), dtype=torch.float32, device=weight.device)
+    ops._check(ops.lib().tllm_fp8_weight(ops._p(weight), ops._dt(weight), ops._p(q), ops._p(scales), n, k, int(gated), ops._stream()), "fp8_weight")
+    return Fp8Weight(q, scales, gated)
+
+
+def quantize_rows_fp8(x: torch.Tensor) -> Fp8Rows:
+    """Rows [T, K] (bfloat16 or float32, K a multiple of 16) in 8 bits."""
+    ops = _ops()
+    _here(x)
+    if x.dim() != 2:
+        _refuse(f"rows are a matrix, got {tuple(x.shape)}")
+    _columns(x.shape[1])
+    out = _empty_rows(x.shape[0], x.shape[1], x.device)
+    ops._check(ops.lib().tllm_fp8_rows(ops._p(x), ops._dt(x), ops._p(out.q), ops._p(out.scales), x.shape[0], x.shape[1], ops._stream()), "fp8_rows")
+    return out
+
+
+def add_rmsnorm_fp8(h: torch.Tensor, delta: Optional[torch.Tensor], gain: torch.Tensor, eps: float) -> Fp8Rows:
+    """``add_rmsnorm`` whose output rows come out in 8 bits, rounded from float32: h += delta (float32, written back), then
+    gain * h / sqrt(mean(h^2) + eps).  Widths that are multiples of 16 up to 32768."""
+    ops = _ops()
+    _here(h, delta, gain)
+    if h.dtype != torch.float32 or h.dim() != 2 or gain.numel() != h.shape[1] or (delta is not None and delta.shape != h.shape):
+        _refuse(f"add_rmsnorm_fp8: stream {h.dtype} {tuple(h.shape)}, delta {None if delta is None else tuple(delta.shape)}, gain {tuple(gain.shape)}")
+    _columns(h.shape[1])
+    out = _empty_rows(h.shape[0], h.shape[1], h.device)
+    ops._check(ops.lib().tllm_add_rmsnorm_fp8(ops._p(h), ops._p(delta), ops.BF16 if delta is None else ops._dt(delta), ops._p(gain), ops._dt(gain),
+                                              float(eps), ops._p(out.q), ops._p(out.scales), h.shape[0], h.shape[1], ops._stream()),
+               "add_rmsnorm_fp8")
+    return out
+
+
+SKINNY_ROWS = 32         # up to this many rows the weight-streaming kernel
+
+
+def _plan(rows: int, n: int, k: int, sms: int):
+    """(columns of a tile, shares of K, blocks per share) of the tensor-core kernel."""
+    kb = _blocks(k)
+    tiles_m = _blocks(rows)
+    if tiles_m * -(-n // 256) >= sms // 2:
+        return 256, 1, kb
+    tiles = tiles_m * _blocks(n)
+    splits = max(1, min(sms // tiles, kb // 2))
+    each = -(-kb // splits)
+    return 128, -(-kb // each), each
+
+
+def _sums(x: Fp8Rows, weight: Fp8Weight, plan):
+    """The product's float32 shares [splits, T, N]."""
+    ops = _ops()
+    rows, k = x.shape
+    n = weight.shape[0]
+    columns, splits, each = plan
+    shares = torch.empty((splits, rows, n), dtype=torch.float32, device=x.device)
+    ops.tcgen05_calls += 1
+    ops._check(ops.lib().tllm_fp8_tcgen05(ops._p(x.q), ops._p(x.scales), ops._p(weight.q), ops._p(weight.scales), ops._p(shares), None, rows, n, k, 1,
+                                          int(weight.gated), columns, splits, each, 0, 0.0, 0.0, ops._p(ops.error_word(x.device)),
+                                          ops._stream()), "fp8_tcgen05")
+    return shares
+
+
+def _check_product(x, weight: Fp8Weight) -> None:
+    if isinstance(x, Fp8Rows):
+        _here(x.q, x.scales, weight.q, weight.scales)
+        if x.q.data_ptr() % 16:
+            _refuse("8-bit rows must be 16-byte aligned")
+    else:
+        _here(x, weight.q, weight.scales)
+        if x.dtype not in (torch.bfloat16, torch.float32) or x.dim() != 2:
+            _refuse(f"a product with an 8-bit weight takes rows in bfloat16, float32 or 8 bits, got {x.dtype} {tuple(x.shape)}")
+        if x.data_ptr() % 16:
+            _refuse("rows must be 16-byte aligned")
+    if x.shape[1] != weight.shape[1]:
+        _refuse(f"rows of {x.shape[1]} columns, a weight of {weight.shape[1]}")
+
+
+def linear_fp8(x, weight: Fp8Weight, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """y[T, N] = x . weight^T: ``x`` bfloat16, float32 (both rounded to 8 bits per 128 columns) or ``Fp8Rows``; bfloat16 or float32 out
+    (default: x's type, bfloat16 for 8-bit rows)."""
+    ops = _ops()
+    _check_product(x, weight)
+    if weight.gated:
+        _refuse("a gated weight belongs to linear_swiglu")
+    want = out_dtype or (x.dtype if x.dtype in ops._DT else torch.bfloat16)
+    if want not in ops._DT:
+        _refuse(f"unsupported dtype {want}")
+    rows, k = x.shape
+    n = weight.shape[0]
+    y = torch.empty((rows, n), dtype=want, device=x.device)
+    if rows == 0:
+        return y
+    if rows <= SKINNY_ROWS:
+        inside = not isinstance(x, Fp8Rows) and x.dtype == torch.bfloat16 and rows <= 8
+        if not inside and not isinstance(x, Fp8Rows):
+            x = quantize_rows_fp8(x)
+        a, s = (x, None) if inside else (x.q, x.scales)
+        ops._check(ops.lib().tllm_fp8_skinny(ops._p(a), ops._p(s), ops._p(weight.q), ops._p(weight.scales), ops._p(y), ops._DT[want], rows, n, k, 0, 0,
+                                             0.0, 0.0, ops._stream()), "fp8_skinny")
+        return y
+    if not isinstance(x, Fp8Rows):
+        x = quantize_rows_fp8(x)
+    plan = _plan(rows, n, k, ops.SM_COUNT)
+    if plan[1] == 1 and want == torch.bfloat16:
+        ops.tcgen05_calls += 1
+        ops._check(ops.lib().tllm_fp8_tcgen05(ops._p(x.q), ops._p(x.scales), ops._p(weight.q), ops._p(weight.scales), ops._p(y), None, rows, n, k, 0, 0,
+                                              plan[0], 1, plan[2], 0, 0.0, 0.0, ops._p(ops.error_word(x.device)), ops._stream()), "fp8_tcgen05")
+        return y
+    shares = _sums(x, weight, plan)
+    ops._check(ops.lib().tllm_fp8_join(ops._p(shares), plan[1], y.numel(), ops._p(y), ops._DT[want], ops._stream()), "fp8_join")
+    return y
+
+
+def linear_swiglu_fp8(x, weight: Fp8Weight, act: str = "silu", consts=None) -> Fp8Rows:
+    """act(x . Wg^T) * (x . Wu^T) for a gated 8-bit weight, as 8-bit rows for the product that follows, rounded from float32."""
+    ops = _ops()
+    _check_product(x, weight)
+    if not weight.gated:
+        _refuse("linear_swiglu takes a gated 8-bit weight (gate and up rows interleaved by eight)")
+    rows, k = x.shape
+    n = weight.shape[0]
+    inter = n // 2
+    _columns(inter)
+    limit, slope = ops._consts(act, consts)
+    code = ops.ACTIVATIONS[act]
+    if rows == 0:
+        return _empty_rows(rows, inter, x.device)
+    if rows <= SKINNY_ROWS:
+        inside = not isinstance(x, Fp8Rows) and x.dtype == torch.bfloat16 and rows <= 8
+        if not inside and not isinstance(x, Fp8Rows):
+            x = quantize_rows_fp8(x)
+        a, s = (x, None) if inside else (x.q, x.scales)
+        y = torch.empty((rows, inter), dtype=torch.float32, device=weight.device)
+        ops._check(ops.lib().tllm_fp8_skinny(ops._p(a), ops._p(s), ops._p(weight.q), ops._p(weight.scales), ops._p(y), ops.F32, rows, inter, k, 1, code,
+                                             limit, slope, ops._stream()), "fp8_skinny")
+        return quantize_rows_fp8(y)
+    if not isinstance(x, Fp8Rows):
+        x = quantize_rows_fp8(x)
+    out = _empty_rows(rows, inter, x.device)
+    plan = _plan(rows, n, k, ops.SM_COUNT)
+    if plan[0] == 256:
+        ops.tcgen05_calls += 1
+        ops._check(ops.lib().tllm_fp8_tcgen05(ops._p(x.q), ops._p(x.scales), ops._p(weight.q), ops._p(weight.scales), ops._p(out.q), ops._p(out.scales),
+                                              rows, n, k, 2, 1, 256, 1, plan[2], code, limit, slope, ops._p(ops.error_word(x.device)),
+                                              ops._stream()), "fp8_tcgen05")
+        return out
+    shares = _sums(x, weight, plan)
+    ops._check(ops.lib().tllm_fp8_gated_rows(ops._p(shares), plan[1], ops._p(out.q), ops._p(out.scales), rows, inter, code, limit, slope, ops._stream()),
+               "fp8_gated_rows")
+    return out
