@@ -9,8 +9,13 @@
 // writes is the rotated query (to `q_out`) or the rotated key / the value (to their
 // page).  Norm sum, angle, sine, cosine and the rotation are float32.
 //
-// Cache layout of one layer: [page][0 = keys, 1 = values][kv head][slot in page][head_dim].
+// Cache layout of one layer: [page][0 = keys, 1 = values][kv head][slot in page][head_dim].  An 8-bit cache (fp8.cuh) has
+// e4m3 keys and values in planes of that shape and a third plane [page][kv head][slot in page][2] of float32 scales, the key's and
+// the value's: one per head of a token, so the lanes that hold the head find it with the shuffles that its norm takes.
+#include <type_traits>
+
 #include "common.cuh"
+#include "fp8.cuh"
 
 namespace tllm {
 
@@ -144,12 +149,17 @@ template <> struct HeadVec8<float> {
 // ROUNDS: how many heads a warp loads before it works on the first.  With many tokens a block of four
 // warps with six loads each in flight keeps more bytes on their way per SM than eight warps with three
 // (the kernel is bound by the latency of its loads, not by its instructions).
-template <typename T, typename TG, int HD, bool TABLE, int ROUNDS>
+// TC: the cache's element type, T or Fp8Planes.
+struct Fp8Planes {
+    uint8_t *k, *v, *scales;
+    long long stride;             // bytes from one page to the next, the same in all three
+};
+template <typename T, typename TG, int HD, bool TABLE, int ROUNDS, typename TC>
 __global__ void __launch_bounds__(256) qk_norm_rope_store_vec_kernel(
     T* qkv, const TG* __restrict__ q_gain, const TG* __restrict__ k_gain, float eps,
     const float* __restrict__ inv_freq, const float* rope_table, const int* __restrict__ positions,
     const int* __restrict__ token_slot, const int* __restrict__ block_table, int max_pages,
-    T* __restrict__ cache, int page_size, T* __restrict__ q_out, int q_heads, int kv_heads, int flags) {
+    TC cache, int page_size, T* __restrict__ q_out, int q_heads, int kv_heads, int flags) {
     constexpr int HALF = HD / 2, LPH = HD / 8, HPW = 32 / LPH;   // lanes per head, heads per warp
     __shared__ __align__(16) float cs[HALF], sn[HALF];
     TLLM_PDL_ENTER();
@@ -251,15 +261,28 @@ __global__ void __launch_bounds__(256) qk_norm_rope_store_vec_kernel(
                     if (is_q || is_k) x[i] = fmaf(x[i], cc[i], other * sx[i]);
                 }
             }
+            float scale8 = 0.0f;
+            if constexpr (std::is_same<TC, Fp8Planes>::value) {
+                float largest = largest8(x);
+#pragma unroll
+                for (int o = LPH / 2; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+                scale8 = fp8_scale(largest);
+            }
             if (!live) continue;
             if (is_q) {
                 if (flags & kFlagQOut) HeadVec8<T>::store(q_out + ((size_t)t * q_heads + head) * HD + e0, x);
             } else {
                 if ((flags & kFlagStore) && page >= 0) {
                     const int kvh = is_k ? head - q_heads : head - q_heads - kv_heads;
-                    T* dst = cache + ((((size_t)page * 2 + (is_k ? 0 : 1)) * kv_heads + kvh) * page_size +
-                                      (pos % page_size)) * HD + e0;
-                    HeadVec8<T>::store(dst, x);
+                    if constexpr (std::is_same<TC, Fp8Planes>::value) {
+                        const size_t token = (size_t)kvh * page_size + pos % page_size, at = (size_t)page * cache.stride;
+                        *reinterpret_cast<uint2*>((is_k ? cache.k : cache.v) + at + token * HD + e0) = to_e4m3x8(x, 1.0f / scale8);
+                        if (l == 0) reinterpret_cast<float*>(cache.scales + at)[token * 2 + (is_k ? 0 : 1)] = scale8;
+                    } else {
+                        T* dst = cache + ((((size_t)page * 2 + (is_k ? 0 : 1)) * kv_heads + kvh) * page_size +
+                                          (pos % page_size)) * HD + e0;
+                        HeadVec8<T>::store(dst, x);
+                    }
                 }
                 if (flags & kFlagKvOut) HeadVec8<T>::store(row + (size_t)head * HD + e0, x);
             }
@@ -326,7 +349,7 @@ extern "C" int tllm_qk_norm_rope_store(
             const bool table = rope_table != nullptr && (flags & kFlagRope) && al(rope_table, 16);
             const bool deep = tokens > 64;                                  // see ROUNDS above
 #define VLAUNCH1(T, TG, HD, TAB, ROUNDS, BLOCK)                                                     \
-    launch_pdl(kPdlQk, qk_norm_rope_store_vec_kernel<T, TG, HD, TAB, ROUNDS>, dim3(tokens, vgroups), dim3(BLOCK), 0, stream, \
+    launch_pdl(kPdlQk, qk_norm_rope_store_vec_kernel<T, TG, HD, TAB, ROUNDS, T*>, dim3(tokens, vgroups), dim3(BLOCK), 0, stream, \
         (T*)qkv, (const TG*)q_gain, (const TG*)k_gain, eps, inv_freq, rope_table, positions, token_slot, \
         block_table, max_pages, (T*)cache, page_size, (T*)q_out, q_heads, kv_heads, flags)
 #define VLAUNCH(T, TG, HD)                                                                          \
@@ -371,4 +394,49 @@ extern "C" int tllm_qk_norm_rope_store(
     }
 #undef LAUNCH
     return finish_launch("qk_norm_rope_store");
+}
+
+// The same into an 8-bit cache: bfloat16 rows, head widths 64 and 128 with no rotation or the whole head rotated.  Planes as Fp8Planes
+// says, keys, values and queries 16-byte aligned, `page_bytes` a multiple of 16.
+extern "C" int tllm_qk_norm_rope_store_fp8(
+    void* qkv, const void* q_gain, const void* k_gain, int gain_dtype, float eps, const float* inv_freq, int rotary_dim,
+    const int* positions, const int* token_slot, const int* block_table, int max_pages, void* k_plane, void* v_plane, void* scales,
+    long long page_bytes, int page_size, void* q_out, int tokens, int q_heads, int kv_heads, int head_dim, int flags,
+    const float* rope_table, cudaStream_t stream) {
+    TLLM_REQUIRE(tokens >= 0 && q_heads > 0 && kv_heads > 0, "qk_norm_rope_store_fp8: bad sizes");
+    TLLM_REQUIRE(head_dim == 64 || head_dim == 128, "qk_norm_rope_store_fp8: head_dim %d is not 64 or 128", head_dim);
+    TLLM_REQUIRE(!(flags & kFlagRope) || (inv_freq != nullptr && rotary_dim == head_dim),
+                 "qk_norm_rope_store_fp8: the whole head rotates or nothing, rotary_dim %d of %d", rotary_dim, head_dim);
+    TLLM_REQUIRE(!(flags & kFlagNorm) || (q_gain && k_gain), "qk_norm_rope_store_fp8: norm without gains");
+    TLLM_REQUIRE(!(flags & kFlagStore) || (k_plane && v_plane && scales && block_table && page_size > 0 && max_pages > 0 && page_bytes > 0),
+                 "qk_norm_rope_store_fp8: store without cache");
+    TLLM_REQUIRE(!(flags & kFlagQOut) || q_out, "qk_norm_rope_store_fp8: no query output");
+    TLLM_REQUIRE(gain_dtype == kBF16 || gain_dtype == kF32, "qk_norm_rope_store_fp8: unknown gain dtype");
+    const auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+    TLLM_REQUIRE(al(qkv) && al(k_plane) && al(v_plane) && al(scales) && al(q_out) && al(rope_table) && page_bytes % 16 == 0,
+                 "qk_norm_rope_store_fp8: operands must be 16-byte aligned");
+    if (tokens == 0) return 0;
+    const Fp8Planes cache{(uint8_t*)k_plane, (uint8_t*)v_plane, (uint8_t*)scales, page_bytes};
+    const int per_block = 8 * (32 / (head_dim / 8));
+    const int vgroups = tokens <= 64 ? (q_heads + 2 * kv_heads + per_block - 1) / per_block : 1;
+    const bool table = rope_table != nullptr && (flags & kFlagRope), deep = tokens > 64;        // see ROUNDS above
+#define STORE8(TG, HD, TAB, ROUNDS, BLOCK)                                                                                            \
+    launch_pdl(kPdlQk, qk_norm_rope_store_vec_kernel<bf16, TG, HD, TAB, ROUNDS, Fp8Planes>, dim3(tokens, vgroups), dim3(BLOCK), 0, stream, \
+               (bf16*)qkv, (const TG*)q_gain, (const TG*)k_gain, eps, inv_freq, rope_table, positions, token_slot, block_table,          \
+               max_pages, cache, page_size, (bf16*)q_out, q_heads, kv_heads, flags)
+#define STORE8_HD(TG, HD)                               \
+    do {                                                \
+        if (table && deep) STORE8(TG, HD, true, 6, 128);\
+        else if (table) STORE8(TG, HD, true, 3, 256);   \
+        else if (deep) STORE8(TG, HD, false, 6, 128);   \
+        else STORE8(TG, HD, false, 3, 256);             \
+    } while (0)
+    if (gain_dtype == kBF16) {
+        if (head_dim == 64) STORE8_HD(bf16, 64); else STORE8_HD(bf16, 128);
+    } else {
+        if (head_dim == 64) STORE8_HD(float, 64); else STORE8_HD(float, 128);
+    }
+#undef STORE8_HD
+#undef STORE8
+    return finish_launch("qk_norm_rope_store_fp8");
 }

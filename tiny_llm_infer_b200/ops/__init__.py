@@ -23,8 +23,8 @@ import torch
 
 from ..csrc import build as _build
 from . import fp8 as _fp8
-from .fp8 import (Fp8Rows, Fp8Weight, add_rmsnorm_fp8, linear_fp8, linear_swiglu_fp8, quantize_rows_fp8,  # noqa: F401
-                  quantize_weight_fp8)
+from .fp8 import (Fp8Rows, Fp8Weight, add_rmsnorm_fp8, linear_fp8, linear_swiglu_fp8, paged_attention_decode_fp8,  # noqa: F401
+                  paged_attention_fp8, qk_norm_rope_store_fp8, quantize_rows_fp8, quantize_weight_fp8)
 
 F32, BF16 = 0, 1
 _DT = {torch.float32: F32, torch.bfloat16: BF16}
@@ -476,6 +476,21 @@ def paged_attention_prefill_tcgen05(q, cache, seg_info, tiles, n_tiles, block_ta
     return out
 
 
+def _attention_tiles(q, cache, block_table, page_size, q_heads, kv_heads, head_dim, window, scale, out, ctx) -> None:
+    """The portions of a step (``ctx.pf_tiles``) on the tensor-core prompt kernels."""
+    if PREFILL_TCGEN05 and head_dim == 128 and getattr(ctx, "n_tiles256", 0):
+        pairs = prefill_tcgen05_block_rows(q_heads, kv_heads) == 128
+        blocks = ctx.n_tiles128 if pairs else ctx.n_tiles256
+        keys = ctx.max_context if not window else min(ctx.max_context, window + 256)
+        splits = prefill_splits(blocks * (q_heads // 2 if pairs else q_heads), keys)
+        paged_attention_prefill_tcgen05(q, cache, ctx.seg_info, ctx.pf_tiles, blocks,
+                                        block_table, page_size, q_heads, kv_heads, head_dim,
+                                        window, scale, out, splits)
+    else:
+        paged_attention_prefill(q, cache, ctx.seg_info, ctx.pf_tiles, ctx.n_tiles, block_table,
+                                page_size, q_heads, kv_heads, head_dim, window, scale, out)
+
+
 def paged_attention(q: torch.Tensor, cache: torch.Tensor, positions, token_slot, block_table,
                     page_size: int, q_heads: int, kv_heads: int, head_dim: int,
                     window: Optional[int], scale: float, out: torch.Tensor, ctx=None) -> torch.Tensor:
@@ -495,17 +510,7 @@ def paged_attention(q: torch.Tensor, cache: torch.Tensor, positions, token_slot,
                                    page_size, q_heads, kv_heads, head_dim, window, scale, out,
                                    ctx.max_context, shared=getattr(ctx, "shared_rows", False))
         if ctx.n_tiles:
-            if PREFILL_TCGEN05 and head_dim == 128 and getattr(ctx, "n_tiles256", 0):
-                pairs = prefill_tcgen05_block_rows(q_heads, kv_heads) == 128
-                blocks = ctx.n_tiles128 if pairs else ctx.n_tiles256
-                keys = ctx.max_context if not window else min(ctx.max_context, window + 256)
-                splits = prefill_splits(blocks * (q_heads // 2 if pairs else q_heads), keys)
-                paged_attention_prefill_tcgen05(q, cache, ctx.seg_info, ctx.pf_tiles, blocks,
-                                                block_table, page_size, q_heads, kv_heads, head_dim,
-                                                window, scale, out, splits)
-            else:
-                paged_attention_prefill(q, cache, ctx.seg_info, ctx.pf_tiles, ctx.n_tiles, block_table,
-                                        page_size, q_heads, kv_heads, head_dim, window, scale, out)
+            _attention_tiles(q, cache, block_table, page_size, q_heads, kv_heads, head_dim, window, scale, out, ctx)
         return out
     rows, n = None, tokens
     if ctx is not None and ctx.pf_tiles is not None and ctx.tokens == tokens and 0 < ctx.n_tiles <= 65535 \

@@ -39,6 +39,10 @@ def declare(h) -> None:
         "tllm_fp8_skinny": [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, f32, f32, vp],
         "tllm_fp8_tcgen05": [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, f32, f32, vp, vp],
         "tllm_fp8_join": [vp, i32, i64, vp, i32, vp],
+        "tllm_qk_norm_rope_store_fp8": [vp, vp, vp, i32, f32, vp, i32, vp, vp, vp, i32, vp, vp, vp, i64, i32, vp, i32, i32, i32, i32, i32,
+                                        vp, vp],
+        "tllm_attention_fp8_decode": [vp, vp, vp, vp, i64, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, f32, i32, vp, vp, vp, vp],
+        "tllm_attention_fp8_unpack": [vp, vp, vp, i64, vp, i32, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp],
     }
     for name, args in sigs.items():
         fn = getattr(h, name)
@@ -310,4 +314,129 @@ def linear_swiglu_fp8(x, weight: Fp8Weight, act: str = "silu", consts=None) -> F
     shares = _sums(x, weight, plan)
     ops._check(ops.lib().tllm_fp8_gated_rows(ops._p(shares), plan[1], ops._p(out.q), ops._p(out.scales), rows, inter, code, limit, slope, ops._stream()),
                "fp8_gated_rows")
+    return out
+
+
+# --------------------------------------------------------------------------- the cache
+SCALE_BYTES = 8          # per token and head: the key's float32 scale, the value's
+
+
+def cache_planes(kv_heads: int, head_dim: int):
+    """The planes (heads, bytes) of an 8-bit cache of keys and values: e4m3 keys, e4m3 values, pairs of float32 scales."""
+    return ((kv_heads, head_dim), (kv_heads, head_dim), (kv_heads, SCALE_BYTES))
+
+
+def cache_takes(page_size: int, q_heads: int, kv_heads: int, head_dim: int) -> bool:
+    """Whether the kernels of the 8-bit cache take these sizes."""
+    return head_dim in (64, 128) and page_size % 16 == 0 and q_heads % kv_heads == 0 and q_heads // kv_heads <= 16
+
+
+def _planes(planes, page_size: int, kv_heads: int, head_dim: int):
+    """(keys, values, scales, bytes from page to page) of an 8-bit cache's planes, checked."""
+    if len(planes) != 3:
+        _refuse(f"an 8-bit cache has planes of keys, values and scales, got {len(planes)}")
+    for plane, width in zip(planes, (head_dim, head_dim, SCALE_BYTES)):
+        if not plane.is_cuda or plane.dtype != torch.uint8 or tuple(plane.shape[1:]) != (kv_heads, page_size, width):
+            _refuse(f"an 8-bit cache's plane is uint8 [pages, {kv_heads}, {page_size}, {width}], got {plane.dtype} {tuple(plane.shape)}")
+        if plane.stride()[1:] != (page_size * width, width, 1) or plane.stride(0) != planes[0].stride(0) or plane.shape[0] != planes[0].shape[0]:
+            _refuse("an 8-bit cache's planes are dense within a page and equally far apart")
+        if plane.device.index != torch.cuda.current_device():
+            _refuse(f"a tensor of {plane.device}, the current device is cuda:{torch.cuda.current_device()}")
+    k, v, s = planes
+    return k.data_ptr(), v.data_ptr(), s.data_ptr(), k.stride(0)
+
+
+def _int32(what: str, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.dtype != torch.int32:
+            _refuse(f"{what}: positions, slots, rows and block tables are int32, got {t.dtype}")
+
+
+def qk_norm_rope_store_fp8(qkv: torch.Tensor, q_gain, k_gain, eps: float, inv_freq, rotary_dim: int, positions: torch.Tensor,
+                           token_slot: torch.Tensor, block_table, planes, page_size: int, q_out, q_heads: int, kv_heads: int, head_dim: int,
+                           flags: int, table: Optional[torch.Tensor] = None) -> None:
+    """``qk_norm_rope_store`` into an 8-bit cache: ``planes`` = (keys, values, scales), ``cache_planes``.  bfloat16 rows, head widths 64 and
+    128, the whole head rotated or nothing."""
+    ops = _ops()
+    _here(qkv, q_gain, k_gain, inv_freq, positions, token_slot, block_table, q_out, table)
+    _int32("qk_norm_rope_store_fp8", positions, token_slot, block_table)
+    tokens = qkv.shape[0]
+    if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != (q_heads + 2 * kv_heads) * head_dim:
+        _refuse(f"qk_norm_rope_store_fp8: rows of {(q_heads + 2 * kv_heads) * head_dim} bfloat16 numbers, got {qkv.dtype} {tuple(qkv.shape)}")
+    if positions.numel() < tokens or token_slot.numel() < tokens:
+        _refuse("qk_norm_rope_store_fp8: a position and a slot for every row")
+    if table is not None and (table.dtype != torch.float32 or tuple(table.shape) != (tokens, 2, rotary_dim // 2)):
+        _refuse(f"qk_norm_rope_store_fp8: rotary table {table.dtype} {tuple(table.shape)}")
+    if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() != rotary_dim // 2):
+        _refuse("qk_norm_rope_store_fp8: a float32 frequency per rotated pair")
+    for gain in (q_gain, k_gain):
+        if gain is not None and gain.numel() != head_dim:
+            _refuse(f"qk_norm_rope_store_fp8: gains of {head_dim} numbers, got {gain.numel()}")
+    if q_gain is not None and k_gain is not None and q_gain.dtype != k_gain.dtype:
+        _refuse("qk_norm_rope_store_fp8: gains of one type")
+    if q_out is not None and (q_out.dtype != torch.bfloat16 or tuple(q_out.shape) != (tokens, q_heads * head_dim)):
+        _refuse(f"qk_norm_rope_store_fp8: queries go to bfloat16 [{tokens}, {q_heads * head_dim}], got {q_out.dtype} {tuple(q_out.shape)}")
+    k, v, s, stride = _planes(planes, page_size, kv_heads, head_dim) if planes is not None else (None, None, None, 0)
+    ops._check(ops.lib().tllm_qk_norm_rope_store_fp8(
+        ops._p(qkv), ops._p(q_gain), ops._p(k_gain), ops._dt(q_gain) if q_gain is not None else ops.F32, float(eps), ops._p(inv_freq), rotary_dim,
+        ops._p(positions), ops._p(token_slot), ops._p(block_table), block_table.shape[1] if block_table is not None else 0, k, v, s, stride, page_size,
+        ops._p(q_out), tokens, q_heads, kv_heads, head_dim, flags, ops._p(table), ops._stream()), "qk_norm_rope_store_fp8")
+
+
+def _attention_operands(what, q, out, positions, token_slot, rows, n_rows, block_table, q_heads, kv_heads, head_dim) -> None:
+    _here(q, out, positions, token_slot, rows, block_table)
+    _int32(what, positions, token_slot, rows, block_table)
+    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or q.dim() != 2 or q.shape[1] != q_heads * head_dim or out.shape != q.shape:
+        _refuse(f"{what}: queries and outputs are bfloat16 [rows, {q_heads * head_dim}], got {q.dtype} {tuple(q.shape)} and {out.dtype} {tuple(out.shape)}")
+    if n_rows > (q.shape[0] if rows is None else rows.numel()) or min(positions.numel(), token_slot.numel()) < q.shape[0]:
+        _refuse(f"{what}: {n_rows} rows of {q.shape[0]}, a position and a slot for each")
+
+
+def paged_attention_decode_fp8(q, planes, positions, token_slot, rows, n_rows, block_table, page_size, q_heads, kv_heads, head_dim, window, scale,
+                               out, max_context, splits=None):
+    """Attention of one-token rows (``rows``: their indices, None for the first ``n_rows``) over an 8-bit paged cache, ``planes`` =
+    (keys, values, scales): positions max(0, pos - window + 1) .. pos of the row's own request.  Keys are split over ``splits`` blocks per
+    (row, key/value head), whose results a second kernel adds in order.  Rows with a negative slot become zeros; rows of ``out``
+    that are not asked for stay as they are.  ``max_context``: no row's position is at or behind it."""
+    ops = _ops()
+    _attention_operands("paged_attention_decode_fp8", q, out, positions, token_slot, rows, n_rows, block_table, q_heads, kv_heads, head_dim)
+    k, v, s, stride = _planes(planes, page_size, kv_heads, head_dim)
+    if max_context > block_table.shape[1] * page_size:
+        max_context = block_table.shape[1] * page_size
+    if splits is None:
+        splits = ops.decode_splits(n_rows, kv_heads, min(max_context, window + 16) if window else max_context)
+    part_o = part_m = None
+    if splits > 1:
+        n = n_rows * q_heads * splits
+        part = torch.empty(n * (head_dim + 3), dtype=torch.float32, device=q.device)
+        part_o, part_m = part[:n * head_dim], part[n * head_dim:]
+    ops._check(ops.lib().tllm_attention_fp8_decode(
+        ops._p(q), k, v, s, stride, ops._p(positions), ops._p(token_slot), ops._p(rows), n_rows, ops._p(block_table), block_table.shape[1], page_size,
+        q_heads, kv_heads, head_dim, int(window or 0), float(scale), splits, ops._p(part_o), ops._p(part_m), ops._p(out), ops._stream()),
+        "paged_attention_decode_fp8", kernels=2 if splits > 1 else 1)
+    return out
+
+
+def paged_attention_fp8(q, planes, positions, token_slot, block_table, page_size, q_heads, kv_heads, head_dim, window, scale, out, ctx=None):
+    """``paged_attention`` over an 8-bit paged cache: one-token rows on ``paged_attention_decode_fp8``; the pages of longer segments are
+    brought back to bfloat16 in scratch, which the prompt kernels read.  Without a context every row is a one-token row."""
+    ops = _ops()
+    tokens = q.shape[0]
+    if ctx is None or ctx.pf_tiles is None or ctx.tokens != tokens:
+        return paged_attention_decode_fp8(q, planes, positions, token_slot, None, tokens, block_table, page_size, q_heads, kv_heads, head_dim, window, scale,
+                                          out, block_table.shape[1] * page_size)
+    if ctx.n_dec:
+        paged_attention_decode_fp8(q, planes, positions, token_slot, ctx.dec_rows, ctx.n_dec, block_table, page_size, q_heads, kv_heads, head_dim,
+                                   window, scale, out, ctx.max_context)
+    if ctx.n_tiles:
+        _attention_operands("paged_attention_fp8", q, out, positions, token_slot, None, tokens, block_table, q_heads, kv_heads, head_dim)
+        k, v, s, stride = _planes(planes, page_size, kv_heads, head_dim)
+        segments, portions = ctx.seg_info.shape[0], ctx.seg_info.shape[0] - ctx.n_dec
+        per = min(-(-ctx.max_context // page_size), block_table.shape[1])
+        pages = torch.empty((portions * per, 2, kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=q.device)
+        table = torch.empty_like(block_table)
+        ops._check(ops.lib().tllm_attention_fp8_unpack(k, v, s, stride, ops._p(ctx.seg_info), segments, ops._p(block_table), block_table.shape[1], page_size,
+                                                       kv_heads, head_dim, portions, per, ops._p(pages), ops._p(table), ops._stream()),
+                   "attention_fp8_unpack")
+        ops._attention_tiles(q, pages, table, page_size, q_heads, kv_heads, head_dim, window, scale, out, ctx)
     return out
