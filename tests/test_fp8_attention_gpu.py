@@ -283,7 +283,8 @@ def test_a_step_of_portions_and_single_tokens(q_heads, kv_heads, dim, page, wind
 
     def dev(x):
         return torch.tensor(x, dtype=torch.int32, device="cuda")
-    ctx = SimpleNamespace(tokens=total, seg_info=dev(seg), dec_rows=dev(dec), n_dec=2, pf_tiles=dev(tiles), n_tiles=len(tiles),
+    segments = [SimpleNamespace(length=n, pos0=p) for _, _, n, p in seg]
+    ctx = SimpleNamespace(tokens=total, segments=segments, seg_info=dev(seg), dec_rows=dev(dec), n_dec=2, pf_tiles=dev(tiles), n_tiles=len(tiles),
                           n_tiles128=sum(t[1] % 128 == 0 for t in tiles), n_tiles256=sum(t[1] % 256 == 0 for t in tiles), max_context=max(lengths))
     out = torch.empty_like(q)
     scale = 1 / math.sqrt(dim)

@@ -52,3 +52,63 @@ def test_tensors_of_the_host_are_refused():
         ops.quantize_weight_fp8(torch.zeros(16, 16))
     with pytest.raises(ops.KernelError):
         ops.linear(torch.zeros(2, 16), ops.Fp8Weight(e4m3(16, 16), torch.ones(1, 1)))
+
+
+def test_only_models_with_the_form_are_taken(tmp_path):
+    """Parts without an 8-bit form, models that are not bfloat16 or not loaded, unknown words: refused in words, on any machine."""
+    from tiny_llm_infer_b200 import LLM
+    from tiny_llm_infer_b200.config.base import describe_model
+    from tiny_llm_infer_b200.engine import load_model
+    from tiny_llm_infer_b200.models.model import Model
+    from tiny import TINIES
+    import tiny_panolorn
+    qwen = Model(describe_model(TINIES["D"]["cfg"]), torch.bfloat16, "cpu")
+    with pytest.raises(ValueError, match="after they are loaded"):
+        qwen.use_fp8_weights()
+    other = Model(describe_model(tiny_panolorn.P1["cfg"]), torch.bfloat16, "cpu")
+    other.loaded = True
+    with pytest.raises(ValueError, match="no 8-bit"):
+        other.use_fp8_weights()
+    with pytest.raises(ValueError, match="no 8-bit cache"):
+        other.use_fp8_cache(16)
+    full = Model(describe_model(TINIES["D"]["cfg"]), torch.float32, "cpu")
+    full.loaded = True
+    with pytest.raises(ValueError):
+        full.use_fp8_weights()
+    with pytest.raises(ValueError):
+        full.use_fp8_cache(16)
+    with pytest.raises(ValueError):
+        qwen.use_fp8_cache(24)
+    with pytest.raises(ValueError, match="int4"):
+        load_model(tmp_path, torch.bfloat16, "cpu", "int4")
+    with pytest.raises(ValueError, match="kv_cache_dtype"):
+        LLM(str(tmp_path), device="cpu", kv_cache_dtype="int8")
+    with pytest.raises(ValueError, match="quantization"):
+        LLM(str(tmp_path), device="cpu", loaded=(qwen, None), quantization="fp8")
+
+
+def test_a_page_of_the_cache_in_bytes():
+    from tiny_llm_infer_b200.cache import CacheManager
+    from tiny_llm_infer_b200.config.base import describe_model
+    from tiny_llm_infer_b200.models.model import Model
+    from tiny import TINIES
+    model = Model(describe_model(TINIES["D"]["cfg"]), torch.bfloat16, "cpu")
+    model.use_fp8_cache(16)
+    sizes = CacheManager.bytes_per_page(model.cache_needs(), 16, torch.uint8)
+    assert sizes == {None: 16 * 2 * (64 + 64 + 8), 80: 16 * 2 * (64 + 64 + 8)}
+    cache = CacheManager(model.cache_needs(), 16, 4, max_slots=2, max_seq_len=64, dtype=torch.uint8, device="cpu")
+    keys, values, scales = cache.view(0).planes
+    assert keys.shape == values.shape == (4, 2, 16, 64) and scales.shape == (4, 2, 16, 8) and keys.stride(0) == scales.stride(0) == 16 * 2 * 136
+    assert (values.data_ptr() - keys.data_ptr(), scales.data_ptr() - keys.data_ptr()) == (2048, 4096)
+
+
+def test_pages_of_portions():
+    from types import SimpleNamespace
+
+    def seg(pos0, length):
+        return SimpleNamespace(pos0=pos0, length=length)
+    ctx = SimpleNamespace(segments=[seg(500, 1), seg(0, 16), seg(15, 2), seg(100, 33)])
+    assert fp8.portion_pages(ctx, 16, None, 40) == (9, 1 + 2 + 9)
+    assert fp8.portion_pages(ctx, 16, 20, 40) == (4, 1 + 2 + 4)      # from the page of 81 to that of 132
+    assert fp8.portion_pages(SimpleNamespace(segments=[seg(5, 1)]), 16, None, 40) == (1, 1)
+    assert fp8.portion_pages(ctx, 16, 20, 40, capturing=True) == (40, 120)

@@ -17,8 +17,8 @@ it prints the same ``run=... output_tokens_per_second=...`` lines.
 
 Added here: ``--prompt-ids`` (requests are token ids; text needs ``--tokenizer``),
 ``--dtype bfloat16|float32``, ``--temperature``, ``--top-p``, ``--seed`` for ``--infer``,
-``--random-weights SEED --config FILE`` (write a random model folder first).  There is no
-``--device cpu`` and no ``--quantization``.
+``--random-weights SEED --config FILE`` (write a random model folder first), ``--quantization fp8``
+and ``--kv-cache-dtype fp8`` (8-bit weights, an 8-bit cache).  There is no ``--device cpu``.
 """
 from __future__ import annotations
 
@@ -43,6 +43,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--prompt-ids", action="append", default=[], help="prompt as comma-separated token ids (repeatable)")
     ap.add_argument("--device", default="cuda", help="cuda or cuda:N")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--quantization", default=None, choices=["fp8"], help="keep the layers' matrices in 8 bits")
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8"], help="keep keys and values in 8 bits")
     ap.add_argument("--max-new-tokens", type=int, default=64)
     ap.add_argument("--max-seq-len", type=int, default=None)
     ap.add_argument("--num-kv-blocks", type=int, default=0)
@@ -125,7 +127,8 @@ def main(argv=None) -> int:
                   max_num_seqs=min(16, len(prompts)),
                   gpu_memory_utilization=args.gpu_memory_utilization or 0.9, device=device,
                   tokenizer=args.tokenizer, enable_prefix_caching=not args.no_prefix_caching,
-                  overlap_scheduling=not args.no_overlap_scheduling, prompt_graphs=args.prompt_graphs)
+                  overlap_scheduling=not args.no_overlap_scheduling, prompt_graphs=args.prompt_graphs,
+                  quantization=args.quantization, kv_cache_dtype=args.kv_cache_dtype)
         params = SamplingParams(max_tokens=args.max_new_tokens, temperature=args.temperature,
                                 top_p=args.top_p, seed=args.seed)
         for result in llm.generate(prompts, params):
@@ -146,7 +149,8 @@ def main(argv=None) -> int:
               block_size=16, max_num_batched_tokens=min(max_seq_len, 256), max_num_seqs=args.num_seqs,
               gpu_memory_utilization=args.gpu_memory_utilization or 0.7, device=device,
               enable_prefix_caching=not args.no_prefix_caching,
-              overlap_scheduling=not args.no_overlap_scheduling, prompt_graphs=args.prompt_graphs)
+              overlap_scheduling=not args.no_overlap_scheduling, prompt_graphs=args.prompt_graphs,
+              quantization=args.quantization, kv_cache_dtype=args.kv_cache_dtype)
     vocab = llm.runner.vocab
     import torch
 

@@ -359,25 +359,30 @@ static int launch_attention_fp8(const void* q, const A8Cache& cache, const int* 
 }
 
 // ---------------------------------------------------------------- pages back in bfloat16
-// For the portions (segments of more than one token) of a step: page i of the j-th portion becomes page j * per + i of `pages`
-// ([pages][keys, values][kv head][token][HD] bfloat16), and table[slot][i] says so, for all pages up to the portion's last token.  The
-// prompt kernels then read those.  One block of threads per (page, portion); bound by HBM.
+// For the portions (segments of more than one token) of a step: the pages that a portion's tokens may read, from the one that holds the
+// first key of its first token's window to the last token's, become pages of `pages` ([pages][keys, values][kv head][token][HD] bfloat16),
+// one portion after the other, and table[slot] lists them (-1 elsewhere).  The prompt kernels then read those.  One block of threads per
+// page; bound by HBM.
 template <int HD>
-__global__ void __launch_bounds__(256) attention_fp8_unpack_kernel(const A8Cache cache, const int* __restrict__ seg_info, int segments,
+__global__ void __launch_bounds__(256) attention_fp8_unpack_kernel(const A8Cache cache, const int* __restrict__ seg_info,
                                                                    const int* __restrict__ block_table, int max_pages, int page_size,
-                                                                   int kv_heads, int per, int portions, bf16* __restrict__ pages,
+                                                                   int kv_heads, int window, int capacity, bf16* __restrict__ pages,
                                                                    int* __restrict__ table) {
     TLLM_PDL_ENTER();
-    const int seg = blockIdx.y, i = blockIdx.x;
-    const int slot = seg_info[4 * seg], length = seg_info[4 * seg + 2], last = seg_info[4 * seg + 3] + length - 1;
+    const int seg = blockIdx.y;
+    const int slot = seg_info[4 * seg], length = seg_info[4 * seg + 2], pos0 = seg_info[4 * seg + 3], last = pos0 + length - 1;
     if (slot < 0 || length <= 1) return;
-    if (i == 0)                                                    // pages behind the last token: none
-        for (int n = last / page_size + 1 + threadIdx.x; n < max_pages; n += blockDim.x) table[(size_t)slot * max_pages + n] = -1;
-    if (i > last / page_size) return;
-    int j = 0;
-    for (int s = 0; s < seg; ++s) j += seg_info[4 * s + 2] > 1 && seg_info[4 * s] >= 0;
-    if (j >= portions) return;
-    const int page = block_table[(size_t)slot * max_pages + i], to = j * per + i;
+    auto first_page = [&](int p) { return window > 0 && p - window + 1 > 0 ? (p - window + 1) / page_size : 0; };
+    const int first = first_page(pos0), i = first + blockIdx.x;
+    if (blockIdx.x == 0)                                           // pages outside: none
+        for (int n = threadIdx.x; n < max_pages; n += blockDim.x)
+            if (n < first || n > last / page_size) table[(size_t)slot * max_pages + n] = -1;
+    if (i > last / page_size || i >= max_pages) return;
+    int to = blockIdx.x;
+    for (int s = 0; s < seg; ++s)
+        if (seg_info[4 * s + 2] > 1 && seg_info[4 * s] >= 0)
+            to += (seg_info[4 * s + 3] + seg_info[4 * s + 2] - 1) / page_size - first_page(seg_info[4 * s + 3]) + 1;
+    const int page = to < capacity ? block_table[(size_t)slot * max_pages + i] : -1;
     if (threadIdx.x == 0) table[(size_t)slot * max_pages + i] = page < 0 ? -1 : to;
     if (page < 0) return;
     const size_t at = (size_t)page * cache.stride, plane = (size_t)kv_heads * page_size;
@@ -440,21 +445,21 @@ extern "C" int tllm_attention_fp8_decode(const void* q, const void* k, const voi
                                                       window, scale, splits, part_o, part_m, out, stream);
 }
 
-// seg_info [segments][4] = slot, first row, tokens, position of the first.  `portions`: how many segments have more than one token;
-// `per`: pages set aside for each; pages bfloat16 [portions * per][2][kv_heads][page_size][head_dim]; table int32 like block_table.
+// seg_info [segments][4] = slot, first row, tokens, position of the first.  `per`: pages of the portion that has most; pages bfloat16
+// [capacity][2][kv_heads][page_size][head_dim], room for all portions' pages; table int32 like block_table.
 extern "C" int tllm_attention_fp8_unpack(const void* k, const void* v, const void* scales, long long page_bytes, const int* seg_info, int segments,
-                                         const int* block_table, int max_pages, int page_size, int kv_heads, int head_dim, int portions, int per,
-                                         void* pages, int* table, cudaStream_t stream) {
+                                         const int* block_table, int max_pages, int page_size, int kv_heads, int head_dim, int window, int per,
+                                         int capacity, void* pages, int* table, cudaStream_t stream) {
     if (check_a8("attention_fp8_unpack", k, v, scales, page_bytes, page_size, kv_heads, head_dim) != 0) return -1;
-    TLLM_REQUIRE(segments > 0 && segments <= 65535 && portions > 0 && per > 0 && per <= max_pages, "attention_fp8_unpack: bad sizes");
+    TLLM_REQUIRE(segments > 0 && segments <= 65535 && per > 0 && per <= max_pages && capacity > 0, "attention_fp8_unpack: bad sizes");
     TLLM_REQUIRE(seg_info && block_table && pages && table && (reinterpret_cast<uintptr_t>(pages) & 15u) == 0, "attention_fp8_unpack: missing operands");
-    TLLM_REQUIRE((long long)2 * kv_heads * page_size * (head_dim / 16) <= 0x7fffffff && (long long)portions * per <= 0x7fffffff, "attention_fp8_unpack: too large");
+    TLLM_REQUIRE((long long)2 * kv_heads * page_size * (head_dim / 16) <= 0x7fffffff, "attention_fp8_unpack: too large");
     const A8Cache cache{(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)scales, page_bytes};
     if (head_dim == 64)
-        launch_pdl(kPdlOther, attention_fp8_unpack_kernel<64>, dim3(per, segments), dim3(256), 0, stream, cache, seg_info, segments, block_table, max_pages,
-                   page_size, kv_heads, per, portions, (bf16*)pages, table);
+        launch_pdl(kPdlOther, attention_fp8_unpack_kernel<64>, dim3(per, segments), dim3(256), 0, stream, cache, seg_info, block_table, max_pages,
+                   page_size, kv_heads, window, capacity, (bf16*)pages, table);
     else
-        launch_pdl(kPdlOther, attention_fp8_unpack_kernel<128>, dim3(per, segments), dim3(256), 0, stream, cache, seg_info, segments, block_table, max_pages,
-                   page_size, kv_heads, per, portions, (bf16*)pages, table);
+        launch_pdl(kPdlOther, attention_fp8_unpack_kernel<128>, dim3(per, segments), dim3(256), 0, stream, cache, seg_info, block_table, max_pages,
+                   page_size, kv_heads, window, capacity, (bf16*)pages, table);
     return finish_launch("attention_fp8_unpack");
 }

@@ -264,7 +264,10 @@ def estimate_num_kv_blocks(model, block_size: int, dtype: torch.dtype, max_num_b
         raise ValueError("gpu_memory_utilization must be in (0, 0.95]")
     free, total = memory if memory is not None else torch.cuda.mem_get_info(device)
     used = total - free
-    per_page = sum(CacheManager.bytes_per_page(model.cache_needs(), block_size, dtype).values())
+    needs = model.cache_needs()
+    per_page = sum(CacheManager.bytes_per_page(needs, block_size, dtype).values())
+    if dtype == torch.uint8:                     # an 8-bit cache: a step's portions may read every page of one layer in bfloat16
+        per_page += max((2 * spec.elements_per_token * block_size for spec, _ in needs.values() if spec is not None), default=0)
     workspace = 4 * model.workspace_floats(max_num_batched_tokens, min(max_num_seqs, max_num_batched_tokens))
     reserve = max(256 << 20, total // 20, workspace)
     states = 0                                   # fixed-size state of every mixer that keeps one, per request slot
@@ -294,6 +297,10 @@ class LLM:
     whose rows only the cache joins (``ModelRunner.ROWS_GRAPH_MAX``), whose rows then go through the
     kernels of one-token rows: their logits differ from those without graphs in rounding.  ``prompt_graphs``
     (off): larger steps with prompt portions whose layout repeats too (faster prompts, slightly slower decoding afterwards).
+    ``quantization`` "fp8": the layers' matrices are kept in 8 bits (e4m3, a float32 scale per block of 128 x 128) and meet rows rounded
+    to 8 bits per 128 columns; embedding, norms and head stay in bfloat16.  ``kv_cache_dtype`` "fp8": keys and values are kept in
+    8 bits, a float32 scale per token and head, half the memory and half the reading.  Both are for bfloat16 models of the
+    architectures whose parts have the form (Qwen3); others are refused.
     """
 
     def __init__(self, model: str, dtype: str = "bfloat16", max_model_len: int = 2048,
@@ -301,24 +308,32 @@ class LLM:
                  max_num_seqs: int = 16, gpu_memory_utilization: float = 0.9, device: str = "cuda:0",
                  tokenizer: Optional[str] = None, loaded=None, use_cuda_graphs: bool = True,
                  enable_prefix_caching: bool = True, overlap_scheduling: bool = True,
-                 prompt_graphs: bool = False):
+                 prompt_graphs: bool = False, quantization: Optional[str] = None, kv_cache_dtype: str = "auto"):
+        if kv_cache_dtype not in ("auto", "fp8"):
+            raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r} is neither 'auto' nor 'fp8'")
+        if loaded is not None and quantization is not None:
+            raise ValueError("a model that is loaded already has its weights: quantization is for model folders")
         if device.startswith("cuda") and not torch.cuda.is_available():
             raise RuntimeError("no CUDA device; this engine has no CPU path")
         torch_dtype = DTYPES[dtype] if isinstance(dtype, str) else dtype
-        self.model, self.model_config = loaded if loaded is not None else load_model(model, torch_dtype, device)
+        self.model, self.model_config = loaded if loaded is not None else load_model(model, torch_dtype, device, quantization)
         max_model_len = min(int(max_model_len), self.model.desc.max_positions)
         block_size = min(int(block_size), max_model_len)
+        cache_dtype = torch_dtype
+        if kv_cache_dtype == "fp8":
+            self.model.use_fp8_cache(block_size)
+            cache_dtype = torch.uint8
         if max_num_batched_tokens is None:
             max_num_batched_tokens = min(max_model_len, 256)
         if num_kv_blocks <= 0:
-            num_kv_blocks = estimate_num_kv_blocks(self.model, block_size, torch_dtype, max_num_batched_tokens,
+            num_kv_blocks = estimate_num_kv_blocks(self.model, block_size, cache_dtype, max_num_batched_tokens,
                                                    gpu_memory_utilization, device, max_num_seqs)
             cap = -(-max_model_len // block_size) * max_num_seqs
             num_kv_blocks = min(num_kv_blocks, cap)
             if num_kv_blocks <= 0:
                 raise RuntimeError("no memory left for the key/value cache")
         self.cache = CacheManager(self.model.cache_needs(), block_size, num_kv_blocks, max_num_seqs,
-                                  max_model_len, torch_dtype, device, prefix_cache=enable_prefix_caching)
+                                  max_model_len, cache_dtype, device, prefix_cache=enable_prefix_caching)
         self.runner = ModelRunner(self.model, self.cache, max_num_batched_tokens, use_graphs=use_cuda_graphs,
                                   prompt_graphs=prompt_graphs)
         self.tokenizer = None

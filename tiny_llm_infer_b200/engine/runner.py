@@ -43,13 +43,21 @@ def strict_float32() -> None:
         torch.backends.cuda.matmul.allow_bf16_reduced_precision_reduction = False
 
 
-def load_model(model_path, dtype: torch.dtype, device) -> Tuple[Model, ModelConfig]:
-    """Model folder (config.json + safetensors) -> model with weights on ``device``."""
+QUANTIZATIONS = ("fp8",)
+
+
+def load_model(model_path, dtype: torch.dtype, device, quantization: Optional[str] = None) -> Tuple[Model, ModelConfig]:
+    """Model folder (config.json + safetensors) -> model with weights on ``device``; ``quantization`` "fp8": the blocks'
+    matrices in 8 bits (``Model.use_fp8_weights``)."""
+    if quantization is not None and quantization not in QUANTIZATIONS:
+        raise ValueError(f"quantization {quantization!r} is not one of {', '.join(QUANTIZATIONS)}")
     config = load_config(model_path)
     desc = describe_model(config)
     model = Model(desc, dtype, device)
     expected, ignorable = expected_tensors(desc)
     model.load(load_weights(model_path, expected, dtype, device, ignorable))
+    if quantization is not None:
+        model.use_fp8_weights()
     return model, config
 
 

@@ -85,6 +85,26 @@ class Model:
             self.head.tie(self.embedding)
         self.loaded = True
 
+    # ---- 8 bits
+    def use_fp8_weights(self) -> None:
+        """Keep the matrices of every block in 8 bits (once, after ``load``).  Embedding, norms and head stay as they are.  A block or
+        a part without that form is refused, and then nothing has changed its form that could still be run: build the model anew."""
+        if not self.loaded:
+            raise ValueError("weights are brought to 8 bits after they are loaded")
+        if self.dtype != torch.bfloat16:
+            raise ValueError(f"8-bit weights are for bfloat16 models, this one is {self.dtype}")
+        for block in self.blocks:
+            block.use_fp8_weights()
+
+    def use_fp8_cache(self, page_size: int) -> None:
+        """Keep keys and values in 8 bits; the cache manager is then made with ``dtype=torch.uint8``."""
+        mixers = [m for b in self.blocks for m in b.mixers()]
+        for mixer in mixers:
+            if not hasattr(mixer, "use_fp8_cache"):
+                raise ValueError(f"{type(mixer).__name__} has no 8-bit cache")
+        for mixer in mixers:
+            mixer.use_fp8_cache(page_size)
+
     # ---- what the cache manager must provide, per cache id
     def cache_needs(self) -> Dict[int, Tuple[Optional[CacheSpec], Optional[StateSpec]]]:
         needs: Dict[int, Tuple[Optional[CacheSpec], Optional[StateSpec]]] = {}

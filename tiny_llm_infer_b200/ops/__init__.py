@@ -22,7 +22,7 @@ from typing import Optional
 import torch
 
 from ..csrc import build as _build
-from . import fp8 as _fp8
+from . import fp8
 from .fp8 import (Fp8Rows, Fp8Weight, add_rmsnorm_fp8, linear_fp8, linear_swiglu_fp8, paged_attention_decode_fp8,  # noqa: F401
                   paged_attention_fp8, qk_norm_rope_store_fp8, quantize_rows_fp8, quantize_weight_fp8)
 
@@ -142,7 +142,7 @@ def _declare(h) -> None:
         fn = getattr(h, name)
         fn.argtypes = args
         fn.restype = i32
-    _fp8.declare(h)
+    fp8.declare(h)
     h.tllm_delta_rule_lanes.argtypes = [i32]
     h.tllm_delta_rule_lanes.restype = i32
     h.tllm_delta_rule_state_floats.argtypes = [i32, i32, i32, i32, i32]

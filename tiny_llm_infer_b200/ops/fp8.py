@@ -42,7 +42,7 @@ def declare(h) -> None:
         "tllm_qk_norm_rope_store_fp8": [vp, vp, vp, i32, f32, vp, i32, vp, vp, vp, i32, vp, vp, vp, i64, i32, vp, i32, i32, i32, i32, i32,
                                         vp, vp],
         "tllm_attention_fp8_decode": [vp, vp, vp, vp, i64, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, f32, i32, vp, vp, vp, vp],
-        "tllm_attention_fp8_unpack": [vp, vp, vp, i64, vp, i32, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp],
+        "tllm_attention_fp8_unpack": [vp, vp, vp, i64, vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp],
     }
     for name, args in sigs.items():
         fn = getattr(h, name)
@@ -417,6 +417,19 @@ def paged_attention_decode_fp8(q, planes, positions, token_slot, rows, n_rows, b
     return out
 
 
+def portion_pages(ctx, page_size: int, window: Optional[int], most: int, capturing: bool = False):
+    """(pages of the portion that has most, pages of all portions) that a step's portions may read, none more than ``most``.  A step that
+    is being captured is replayed with other portions of as many tokens: room for the most."""
+    counts = [1]
+    for s in ctx.segments:
+        if s.length > 1:
+            first = max(0, s.pos0 - window + 1) if window else 0
+            counts.append((s.pos0 + s.length - 1) // page_size - first // page_size + 1)
+    if capturing:
+        return most, most * max(1, len(counts) - 1)
+    return max(counts), max(1, sum(counts) - 1)
+
+
 def paged_attention_fp8(q, planes, positions, token_slot, block_table, page_size, q_heads, kv_heads, head_dim, window, scale, out, ctx=None):
     """``paged_attention`` over an 8-bit paged cache: one-token rows on ``paged_attention_decode_fp8``; the pages of longer segments are
     brought back to bfloat16 in scratch, which the prompt kernels read.  Without a context every row is a one-token row."""
@@ -431,12 +444,12 @@ def paged_attention_fp8(q, planes, positions, token_slot, block_table, page_size
     if ctx.n_tiles:
         _attention_operands("paged_attention_fp8", q, out, positions, token_slot, None, tokens, block_table, q_heads, kv_heads, head_dim)
         k, v, s, stride = _planes(planes, page_size, kv_heads, head_dim)
-        segments, portions = ctx.seg_info.shape[0], ctx.seg_info.shape[0] - ctx.n_dec
-        per = min(-(-ctx.max_context // page_size), block_table.shape[1])
-        pages = torch.empty((portions * per, 2, kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=q.device)
+        segments, most = ctx.seg_info.shape[0], min(-(-ctx.max_context // page_size), block_table.shape[1])
+        per, capacity = portion_pages(ctx, page_size, window, most, torch.cuda.is_current_stream_capturing())
+        pages = torch.empty((capacity, 2, kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=q.device)
         table = torch.empty_like(block_table)
         ops._check(ops.lib().tllm_attention_fp8_unpack(k, v, s, stride, ops._p(ctx.seg_info), segments, ops._p(block_table), block_table.shape[1], page_size,
-                                                       kv_heads, head_dim, portions, per, ops._p(pages), ops._p(table), ops._stream()),
+                                                       kv_heads, head_dim, int(window or 0), per, capacity, ops._p(pages), ops._p(table), ops._stream()),
                    "attention_fp8_unpack")
         ops._attention_tiles(q, pages, table, page_size, q_heads, kv_heads, head_dim, window, scale, out, ctx)
     return out

@@ -47,6 +47,7 @@ class GroupedQueryAttention:
             if getattr(self.position, "pairs", False):
                 raise ValueError(f"position encoding {position.kind!r} turns neighbouring elements, this part's kernel halves")
         self.w_qkv = self.w_o = self.q_gain = self.k_gain = None
+        self.cache_fp8 = False
 
     # ---- weights
     @classmethod
@@ -72,8 +73,25 @@ class GroupedQueryAttention:
             gd = torch.float32 if any(g.dtype == torch.float32 for g in gains) else gains[0].dtype
             self.q_gain, self.k_gain = (g.to(gd).contiguous() for g in gains)
 
+    def use_fp8_weights(self) -> None:
+        """The four projections as e4m3 values with scales."""
+        if self.hidden % 16 or self.q_heads * self.head_dim % 16:
+            raise ValueError(f"8-bit weights need widths that are multiples of 16: model {self.hidden}, heads {self.q_heads * self.head_dim}")
+        self.w_qkv, self.w_o = ops.quantize_weight_fp8(self.w_qkv), ops.quantize_weight_fp8(self.w_o)
+
+    def use_fp8_cache(self, page_size: int) -> None:
+        """Keys and values as e4m3 with a scale per token and head (``ops.fp8.cache_planes``)."""
+        fused = self.position is None or (hasattr(self.position, "fused_rotary") and (self.position.fused_rotary() or (None, None))[1] == self.head_dim)
+        if self.dtype != torch.bfloat16 or not fused or not ops.fp8.cache_takes(page_size, self.q_heads, self.kv_heads, self.head_dim):
+            raise ValueError(f"an 8-bit cache is for bfloat16 models, heads of 64 or 128 that turn whole, at most 16 query heads per key/value "
+                             f"head and pages of a multiple of 16 tokens: {self.dtype}, {self.q_heads} and {self.kv_heads} heads of "
+                             f"{self.head_dim}, pages of {page_size}")
+        self.cache_fp8 = True
+
     # ---- what the cache manager has to provide
     def cache_spec(self) -> Optional[CacheSpec]:
+        if self.cache_fp8:
+            return CacheSpec(ops.fp8.cache_planes(self.kv_heads, self.head_dim), self.window)
         return CacheSpec.keys_and_values(self.kv_heads, self.head_dim, self.window)
 
     def state_spec(self) -> Optional[StateSpec]:
@@ -90,6 +108,16 @@ class GroupedQueryAttention:
         norm = ops.QK_NORM if self.qk_norm_eps is not None else 0
         store = ops.QK_STORE if cache.writes else 0
         eps = self.qk_norm_eps if self.qk_norm_eps is not None else 1.0
+        if self.cache_fp8:
+            inv_freq, rotary_dim = self.position.fused_rotary() if self.position is not None else (None, 0)
+            table = self.position.step_table(ctx) if self.position is not None and hasattr(self.position, "step_table") else None
+            ops.qk_norm_rope_store_fp8(qkv, self.q_gain, self.k_gain, eps, inv_freq, rotary_dim, ctx.positions, ctx.token_slot,
+                                       cache.block_table, cache.planes, cache.page_size, q, self.q_heads, self.kv_heads, self.head_dim,
+                                       norm | (ops.QK_ROPE if rotary_dim else 0) | store | ops.QK_QOUT, table)
+            out = torch.empty_like(q)
+            ops.paged_attention_fp8(q, cache.planes, ctx.positions, ctx.token_slot, cache.block_table, cache.page_size, self.q_heads,
+                                    self.kv_heads, self.head_dim, self.window, self.scale, out, ctx)
+            return ops.linear(out, self.w_o, out_dtype=self.dtype)
         args = dict(positions=ctx.positions, token_slot=ctx.token_slot, block_table=cache.block_table,
                     cache=cache.kv, page_size=cache.page_size, q_out=q, q_heads=self.q_heads,
                     kv_heads=self.kv_heads, head_dim=self.head_dim)

@@ -69,6 +69,10 @@ class Block:
         each a cache of its own)."""
         return [self.parts[role] for role, category in self.roles.items() if category == "mixer"]
 
+    def use_fp8_weights(self) -> None:
+        """Keep the sub-layers' matrices in 8 bits, and have the norms hand their rows on in 8 bits."""
+        raise ValueError(f"blocks of kind {type(self).__name__} have no 8-bit weights")
+
 
 @register("block", "prenorm")
 class PreNormBlock(Block):
@@ -80,6 +84,14 @@ class PreNormBlock(Block):
         a = self.mixer.forward(x, ctx, cache)
         x = self.norm2.forward(h, a)
         return self.ffn.forward(x, ctx)
+
+    def use_fp8_weights(self) -> None:
+        for role, part in self.parts.items():
+            if not hasattr(part, "use_fp8_weights" if self.roles[role] != "norm" else "rows_fp8"):
+                raise ValueError(f"{type(part).__name__} has no 8-bit form")
+        self.mixer.use_fp8_weights()
+        self.ffn.use_fp8_weights()
+        self.norm1.rows_fp8 = self.norm2.rows_fp8 = True
 
 
 @register("block", "sandwich")

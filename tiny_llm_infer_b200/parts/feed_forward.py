@@ -52,10 +52,20 @@ class SwiGLUFeedForward:
             self.w_gate_up = torch.cat([p.to(common) for p in parts], dim=0).contiguous()
         self.w_down = t[self.names[2]].contiguous()
 
+    def use_fp8_weights(self) -> None:
+        """Gate and up, and down, as e4m3 values with scales; the activation leaves its product as 8-bit rows."""
+        if self.hidden % 16 or self.inter % 16:
+            raise ValueError(f"8-bit weights need widths that are multiples of 16: model {self.hidden}, feed-forward {self.inter}")
+        self.w_gate_up = ops.quantize_weight_fp8(self.w_gate_up, gated=True)
+        self.w_down = ops.quantize_weight_fp8(self.w_down)
+
     def workspace_floats(self, tokens: int) -> int:
         return 3 * tokens * self.inter          # the product of gate and up, and the activation
 
     def forward(self, x: torch.Tensor, ctx) -> torch.Tensor:
+        if isinstance(self.w_gate_up, ops.Fp8Weight):
+            act = ops.linear_swiglu(x, self.w_gate_up, act=self.activation, consts=self.act_consts)
+            return ops.linear(act, self.w_down, out_dtype=self.dtype)
         act = ops.linear_swiglu(x, self.w_gate_up, out_dtype=self.dtype, interleaved=self.interleaved,
                                 act=self.activation, consts=self.act_consts)
         return ops.linear(act, self.w_down, out_dtype=self.dtype)

@@ -53,6 +53,7 @@ class RMSNorm:
                  offset: float = 0.0, float32_gain: bool = False):
         self.width, self.eps, self.dtype, self.device = int(width), float(eps), dtype, device
         self.name, self.offset, self.float32_gain = name, float(offset), bool(float32_gain)
+        self.rows_fp8 = False          # rows for products with 8-bit weights: in 8 bits, rounded from float32
         self.gain: Optional[torch.Tensor] = None
 
     @classmethod
@@ -78,6 +79,8 @@ class RMSNorm:
         return ops.sum_rmsnorm(h, list(deltas), list(coefs), alpha, self.gain, self.eps, out, bias=bias)
 
     def forward(self, h: torch.Tensor, delta, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if self.rows_fp8 and rows is None and (delta is None or isinstance(delta, torch.Tensor)):
+            return ops.add_rmsnorm_fp8(h, delta, self.gain, self.eps)
         n = h.shape[0] if rows is None else rows.numel()
         out = torch.empty((n, self.width), dtype=self.dtype, device=h.device)
         if isinstance(delta, StreamCopy):
