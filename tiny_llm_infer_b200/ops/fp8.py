@@ -198,7 +198,8 @@ def add_rmsnorm_fp8(h: torch.Tensor, delta: Optional[torch.Tensor], gain: torch.
     return out
 
 
-SKINNY_ROWS = 32         # up to this many rows the weight-streaming kernel
+SKINNY_ROWS = 16         # up to this many rows the weight-streaming kernel
+SKINNY_INSIDE_K = 4096   # up to this many columns it rounds eight bfloat16 rows itself
 
 
 def _plan(rows: int, n: int, k: int, sms: int):
@@ -258,7 +259,7 @@ def linear_fp8(x, weight: Fp8Weight, out_dtype: Optional[torch.dtype] = None) ->
     if rows == 0:
         return y
     if rows <= SKINNY_ROWS:
-        inside = not isinstance(x, Fp8Rows) and x.dtype == torch.bfloat16 and rows <= 8
+        inside = not isinstance(x, Fp8Rows) and x.dtype == torch.bfloat16 and rows <= 8 and k <= SKINNY_INSIDE_K
         if not inside and not isinstance(x, Fp8Rows):
             x = quantize_rows_fp8(x)
         a, s = (x, None) if inside else (x.q, x.scales)
@@ -293,7 +294,7 @@ def linear_swiglu_fp8(x, weight: Fp8Weight, act: str = "silu", consts=None) -> F
     if rows == 0:
         return _empty_rows(rows, inter, x.device)
     if rows <= SKINNY_ROWS:
-        inside = not isinstance(x, Fp8Rows) and x.dtype == torch.bfloat16 and rows <= 8
+        inside = not isinstance(x, Fp8Rows) and x.dtype == torch.bfloat16 and rows <= 8 and k <= SKINNY_INSIDE_K
         if not inside and not isinstance(x, Fp8Rows):
             x = quantize_rows_fp8(x)
         a, s = (x, None) if inside else (x.q, x.scales)
