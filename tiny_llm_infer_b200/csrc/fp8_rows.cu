@@ -201,9 +201,9 @@ extern "C" int tllm_fp8_rows(const void* x, int dtype, void* q, float* scales, i
     const long long blocks = (long long)rows * kb, grid = (blocks + 15) / 16;
     TLLM_REQUIRE(grid <= 0x7fffffff, "fp8_rows: too many rows");
     if (dtype == kF32)
-        launch_pdl(kPdlOther, fp8_rows_kernel<float>, dim3((unsigned)grid), dim3(256), 0, stream, (const float*)x, (uint8_t*)q, scales, K, kb, blocks);
+        launch_pdl(kPdlAlways, fp8_rows_kernel<float>, dim3((unsigned)grid), dim3(256), 0, stream, (const float*)x, (uint8_t*)q, scales, K, kb, blocks);
     else
-        launch_pdl(kPdlOther, fp8_rows_kernel<bf16>, dim3((unsigned)grid), dim3(256), 0, stream, (const bf16*)x, (uint8_t*)q, scales, K, kb, blocks);
+        launch_pdl(kPdlAlways, fp8_rows_kernel<bf16>, dim3((unsigned)grid), dim3(256), 0, stream, (const bf16*)x, (uint8_t*)q, scales, K, kb, blocks);
     return finish_launch("fp8_rows");
 }
 
@@ -218,7 +218,7 @@ extern "C" int tllm_fp8_gated_rows(const float* sums, int splits, void* q, float
     const int ib = (inter + kFp8Block - 1) / kFp8Block;
     const long long blocks = (long long)rows * ib, grid = (blocks + 15) / 16;
     TLLM_REQUIRE(grid <= 0x7fffffff, "fp8_gated_rows: too many rows");
-    launch_pdl(kPdlOther, fp8_gated_rows_kernel, dim3((unsigned)grid), dim3(256), 0, stream, sums, splits, (long long)rows * inter * 2,
+    launch_pdl(kPdlAlways, fp8_gated_rows_kernel, dim3((unsigned)grid), dim3(256), 0, stream, sums, splits, (long long)rows * inter * 2,
                (uint8_t*)q, scales, inter, ib, blocks, act, GateConst{limit, slope});
     return finish_launch("fp8_gated_rows");
 }

@@ -203,15 +203,14 @@ SKINNY_INSIDE_K = 4096   # up to this many columns it rounds eight bfloat16 rows
 
 
 def _plan(rows: int, n: int, k: int, sms: int):
-    """(columns of a tile, shares of K, blocks per share) of the tensor-core kernel."""
+    """(whether pairs of SMs take tiles of 256 x 256, shares of K, blocks per share) of the tensor-core kernels."""
     kb = _blocks(k)
-    tiles_m = _blocks(rows)
-    if tiles_m * -(-n // 256) >= sms // 2:
-        return 256, 1, kb
-    tiles = tiles_m * _blocks(n)
+    if -(-rows // 256) * -(-n // 256) >= sms // 4:
+        return True, 1, kb
+    tiles = _blocks(rows) * _blocks(n)
     splits = max(1, min(sms // tiles, kb // 2))
     each = -(-kb // splits)
-    return 128, -(-kb // each), each
+    return False, -(-kb // each), each
 
 
 def _sums(x: Fp8Rows, weight: Fp8Weight, plan):
@@ -219,11 +218,11 @@ def _sums(x: Fp8Rows, weight: Fp8Weight, plan):
     ops = _ops()
     rows, k = x.shape
     n = weight.shape[0]
-    columns, splits, each = plan
+    _, splits, each = plan
     shares = torch.empty((splits, rows, n), dtype=torch.float32, device=x.device)
     ops.tcgen05_calls += 1
     ops._check(ops.lib().tllm_fp8_tcgen05(ops._p(x.q), ops._p(x.scales), ops._p(weight.q), ops._p(weight.scales), ops._p(shares), None, rows, n, k, 1,
-                                          int(weight.gated), columns, splits, each, 0, 0.0, 0.0, ops._p(ops.error_word(x.device)),
+                                          int(weight.gated), 0, splits, each, 0, 0.0, 0.0, ops._p(ops.error_word(x.device)),
                                           ops._stream()), "fp8_tcgen05")
     return shares
 
@@ -272,7 +271,7 @@ def linear_fp8(x, weight: Fp8Weight, out_dtype: Optional[torch.dtype] = None) ->
     if plan[1] == 1 and want == torch.bfloat16:
         ops.tcgen05_calls += 1
         ops._check(ops.lib().tllm_fp8_tcgen05(ops._p(x.q), ops._p(x.scales), ops._p(weight.q), ops._p(weight.scales), ops._p(y), None, rows, n, k, 0, 0,
-                                              plan[0], 1, plan[2], 0, 0.0, 0.0, ops._p(ops.error_word(x.device)), ops._stream()), "fp8_tcgen05")
+                                              int(plan[0]), 1, plan[2], 0, 0.0, 0.0, ops._p(ops.error_word(x.device)), ops._stream()), "fp8_tcgen05")
         return y
     shares = _sums(x, weight, plan)
     ops._check(ops.lib().tllm_fp8_join(ops._p(shares), plan[1], y.numel(), ops._p(y), ops._DT[want], ops._stream()), "fp8_join")
@@ -306,10 +305,10 @@ def linear_swiglu_fp8(x, weight: Fp8Weight, act: str = "silu", consts=None) -> F
         x = quantize_rows_fp8(x)
     out = _empty_rows(rows, inter, x.device)
     plan = _plan(rows, n, k, ops.SM_COUNT)
-    if plan[0] == 256:
+    if plan[0]:
         ops.tcgen05_calls += 1
         ops._check(ops.lib().tllm_fp8_tcgen05(ops._p(x.q), ops._p(x.scales), ops._p(weight.q), ops._p(weight.scales), ops._p(out.q), ops._p(out.scales),
-                                              rows, n, k, 2, 1, 256, 1, plan[2], code, limit, slope, ops._p(ops.error_word(x.device)),
+                                              rows, n, k, 2, 1, 1, 1, plan[2], code, limit, slope, ops._p(ops.error_word(x.device)),
                                               ops._stream()), "fp8_tcgen05")
         return out
     shares = _sums(x, weight, plan)
