@@ -43,6 +43,15 @@ __device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint
         : "memory");
 }
 
+// A wait by all lanes of a warp in a loop whose length is what the kernel's speed hangs on: unlike warp_wait it does not read the block's
+// flag (some 100 cycles a wait); where another warp has given up, this one's own limit runs out.
+__device__ __forceinline__ bool quick_wait(uint64_t* bar, uint32_t parity, volatile int* aborted, int* error_word, int code) {
+    if (__all_sync(0xffffffffu, mbar_wait(bar, parity))) return true;
+    atomicExch(error_word, code);
+    *aborted = 1;
+    return false;
+}
+
 // What the tile's sums become.
 enum Fp8Out : int { kOutBf16 = 0, kOutShare = 1, kOutGated = 2 };
 
@@ -378,7 +387,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     constexpr bool INTER = OUT == kOutGated;
     constexpr int kCols = 128;                                  // of a summing thread
-    __shared__ __align__(8) uint64_t full_bar[kPairStages], empty_bar[kPairStages], part_full[2], part_empty[2];
+    // a stage's data are there; its MMAs are done (the stage is free again, the block's products are there); a half of tensor memory is read
+    __shared__ __align__(8) uint64_t full_bar[kPairStages], done_bar[kPairStages], part_empty[2];
     __shared__ uint32_t tmem_base_slot;
     __shared__ int abort_flag;
     __shared__ Fp8Meeting meet;
@@ -391,10 +401,9 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     if (threadIdx.x == 0) {
         for (int s = 0; s < kPairStages; ++s) {
             mbar_init(&full_bar[s], 1);
-            mbar_init(&empty_bar[s], 1);
+            mbar_init(&done_bar[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
-            mbar_init(&part_full[b], 1);
             mbar_init(&part_empty[b], 2 * kQSumWarps);          // of both SMs
         }
         for (int q = 0; q < 4; ++q) mbar_init(&meet.bar[q], 2);
@@ -423,7 +432,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 const int row = (t % p.tiles_m) * 256 + rank * 128, col = (t / p.tiles_m) * 256 + rank * 128;
                 for (int kb = 0; kb < p.kb_all; ++kb, ++it) {
                     const int s = it % kPairStages;
-                    if (it >= kPairStages && !mbar_wait(&empty_bar[s], ((it / kPairStages) - 1) & 1)) {
+                    if (it >= kPairStages && !mbar_wait(&done_bar[s], ((it / kPairStages) - 1) & 1)) {
                         atomicExch(error_word, 1);
                         *aborted = 1;
                     }
@@ -440,28 +449,22 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 const int first = it > kPairStages ? it - kPairStages : 0;
                 for (int i = first; i < it; ++i) mbar_wait(&full_bar[i % kPairStages], (i / kPairStages) & 1);
             }
-        } else if (warp == 1 && rank == 0) {
+        } else if ((warp == 1 || warp == 2) && rank == 0) {
+            // two warps issue in turn, one for each half of tensor memory: a warp's waits, issue and commit take as long as a block's MMAs
             constexpr uint32_t idesc = instr_desc_e4m3(256, 256);
-            const uint32_t issue = lane == 0;
-            int it = 0;
-            for (int t = pair; t < total; t += pairs) {
-                bool ok = true;
-                for (int kb = 0; kb < p.kb_all; ++kb, ++it) {
-                    const int s = it % kPairStages, buf = it & 1;
-                    ok = it < 2 || warp_wait(&part_empty[buf], ((it >> 1) - 1) & 1, aborted, error_word, 4);
-                    if (!ok) break;
-                    ok = warp_wait(&full_bar[s], (it / kPairStages) & 1, aborted, error_word, 2);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                    const uint32_t a_addr = cvta_shared(tiles + (size_t)s * kPairStage);
-                    const uint64_t a_desc = smem_desc_sw128(a_addr), b_desc = smem_desc_sw128(a_addr + 128 * kQK);
+            const uint32_t issue = lane == 0, acc = tmem_base + (warp - 1) * 256;
+            const int blocks = (total - pair + pairs - 1) / pairs * p.kb_all;       // of all of this pair's tiles
+            for (int it = warp - 1; it < blocks; it += 2) {
+                const int s = it % kPairStages;
+                if (!quick_wait(&full_bar[s], (it / kPairStages) & 1, aborted, error_word, 2)) break;
+                if (it >= 2 && !quick_wait(&part_empty[warp - 1], ((it >> 1) - 1) & 1, aborted, error_word, 4)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                const uint32_t a_addr = cvta_shared(tiles + (size_t)s * kPairStage);
+                const uint64_t a_desc = smem_desc_sw128(a_addr), b_desc = smem_desc_sw128(a_addr + 128 * kQK);
 #pragma unroll
-                    for (int k = 0; k < kQK / 32; ++k)           // 32 bytes further: two units of the descriptor's address
-                        umma_pair_if(issue, tmem_base + buf * 256, a_desc + 2 * k, b_desc + 2 * k, idesc, k > 0 ? 1u : 0u);
-                    umma_commit_pair_if(issue, &empty_bar[s]);
-                    umma_commit_pair_if(issue, &part_full[buf]);
-                }
-                if (!ok) break;
+                for (int k = 0; k < kQK / 32; ++k)               // 32 bytes further: two units of the descriptor's address
+                    umma_pair_if(issue, acc, a_desc + 2 * k, b_desc + 2 * k, idesc, k > 0 ? 1u : 0u);
+                umma_commit_pair_if(issue, &done_bar[s]);
             }
         }
     } else {
@@ -491,12 +494,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                     s_w = sw[kb + 1];
                     if (INTER) s_u = sw[p.kb_all + kb + 1];
                 }
-                ok = __all_sync(0xffffffffu, mbar_wait(&part_full[buf], (it >> 1) & 1));
-                if (!ok) {
-                    atomicExch(error_word, 3);
-                    *aborted = 1;
-                    break;
-                }
+                ok = quick_wait(&done_bar[it % kPairStages], (it / kPairStages) & 1, aborted, error_word, 3);
+                if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
 #pragma unroll
                 for (int c = 0; c < kCols; c += 64) {
