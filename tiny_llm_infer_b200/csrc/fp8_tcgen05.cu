@@ -25,7 +25,7 @@
 namespace tllm {
 
 constexpr int kQM = 128, kQK = 128;              // tile rows; k's per stage = one scale block = one 128-byte swizzle row
-constexpr int kQSumWarps = 8, kQThreads = (2 + kQSumWarps) * 32;
+constexpr int kQSumWarps = 8, kQThreads = (3 + kQSumWarps) * 32;
 constexpr int kQPad = 64 + 16;                   // bytes of a staging row: 64 of output, padded against bank conflicts
 constexpr uint32_t kQTmemCols = 512;
 constexpr int kQStages = 6;                      // of 32 KB
@@ -34,13 +34,36 @@ constexpr int kQStages = 6;                      // of 32 KB
 __host__ __device__ constexpr uint32_t instr_desc_e4m3(int m, int n) {
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-__device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// Issued by the lane that says so; the warp goes through it as one, its descriptors in uniform registers.
+__device__ __forceinline__ void umma_e4m3_if(uint32_t issue, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(issue)
         : "memory");
+}
+__device__ __forceinline__ void umma_commit_if(uint32_t issue, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(cvta_shared(bar)),
+        "r"(issue)
+        : "memory");
+}
+// Two sums at a time: (a, b) += (x, y) * (s, t).
+__device__ __forceinline__ void fma_pair(float& a, float& b, uint32_t x, uint32_t y, uint64_t st) {
+    uint64_t v, d;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "r"(x), "r"(y));
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(d) : "f"(a), "f"(b));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;\n" : "+l"(d) : "l"(v), "l"(st));
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(d));
+}
+__device__ __forceinline__ uint64_t twice(float s) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %1};\n" : "=l"(d) : "f"(s));
+    return d;
 }
 
 // A wait by all lanes of a warp in a loop whose length is what the kernel's speed hangs on: unlike warp_wait it does not read the block's
@@ -177,7 +200,8 @@ fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     constexpr int BN = 128, kStageA = kQM * kQK, kStageB = BN * kQK, kStage = kStageA + kStageB;
     constexpr int kStages = kQStages, kBufs = 512 / BN;
     constexpr int kCols = BN / 2;                               // of a summing thread
-    __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages], part_full[kBufs], part_empty[kBufs];
+    // a stage's data are there; its MMAs are done (the stage is free again, the block's products are there); a quarter of tensor memory is read
+    __shared__ __align__(8) uint64_t full_bar[kStages], done_bar[kStages], part_empty[kBufs];
     __shared__ uint32_t tmem_base_slot;
     __shared__ int abort_flag;
     unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -187,10 +211,9 @@ fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&full_bar[s], 1);
-            mbar_init(&empty_bar[s], 1);
+            mbar_init(&done_bar[s], 1);
         }
         for (int b = 0; b < kBufs; ++b) {
-            mbar_init(&part_full[b], 1);
             mbar_init(&part_empty[b], kQSumWarps);
         }
         abort_flag = 0;
@@ -223,7 +246,7 @@ fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                 const int n = blocks_of(rest / p.tiles_n, kb0);
                 for (int kb = 0; kb < n; ++kb, ++it) {
                     const int s = it % kStages;
-                    if (it >= kStages && !mbar_wait(&empty_bar[s], ((it / kStages) - 1) & 1)) {
+                    if (it >= kStages && !mbar_wait(&done_bar[s], ((it / kStages) - 1) & 1)) {
                         atomicExch(error_word, 1);
                         *aborted = 1;
                     }
@@ -239,39 +262,35 @@ fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                 for (int i = first; i < it; ++i) mbar_wait(&full_bar[i % kStages], (i / kStages) & 1);
             }
         }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = instr_desc_e4m3(kQM, BN);
-            int it = 0;
-            for (int t = blockIdx.x; t < total && !*aborted; t += gridDim.x) {
-                int kb0;
-                const int n = blocks_of(t / p.tiles_m / p.tiles_n, kb0);
-                for (int kb = 0; kb < n; ++kb, ++it) {
-                    const int s = it % kStages, buf = it % kBufs;
-                    if (it >= kBufs && !mbar_wait(&part_empty[buf], ((it / kBufs) - 1) & 1)) {
-                        atomicExch(error_word, 4);
-                        *aborted = 1;
-                        break;
-                    }
-                    if (!mbar_wait(&full_bar[s], (it / kStages) & 1)) {
-                        atomicExch(error_word, 2);
-                        *aborted = 1;
-                        break;
-                    }
-                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                    const uint32_t a_addr = cvta_shared(tiles + (size_t)s * kStage), b_addr = a_addr + kStageA;
+    } else if (warp < 3) {
+        // two warps issue in turn (see the pairs below)
+        constexpr uint32_t idesc = instr_desc_e4m3(kQM, BN);
+        const uint32_t issue = lane == 0;
+        int it = 0;                                              // blocks of the tiles before
+        bool ok = true;
+        for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
+            int kb0;
+            const int n = blocks_of(t / p.tiles_m / p.tiles_n, kb0);
+            for (int i = it; i < it + n; ++i) {
+                if ((i & 1) != warp - 1) continue;
+                const int s = i % kStages, buf = i % kBufs;
+                ok = quick_wait(&full_bar[s], (i / kStages) & 1, aborted, error_word, 2) &&
+                     (i < kBufs || quick_wait(&part_empty[buf], ((i / kBufs) - 1) & 1, aborted, error_word, 4));
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                const uint32_t a_addr = cvta_shared(tiles + (size_t)s * kStage);
+                const uint64_t a_desc = smem_desc_sw128(a_addr), b_desc = smem_desc_sw128(a_addr + kStageA);
 #pragma unroll
-                    for (int k = 0; k < kQK / 32; ++k)
-                        umma_e4m3(tmem_base + buf * BN, smem_desc_sw128(a_addr + k * 32), smem_desc_sw128(b_addr + k * 32), idesc, k > 0 ? 1u : 0u);
-                    umma_commit(&empty_bar[s]);
-                    umma_commit(&part_full[buf]);
-                }
+                for (int k = 0; k < kQK / 32; ++k)               // 32 bytes further: two units of the descriptor's address
+                    umma_e4m3_if(issue, tmem_base + buf * BN, a_desc + 2 * k, b_desc + 2 * k, idesc, k > 0 ? 1u : 0u);
+                umma_commit_if(issue, &done_bar[s]);
             }
+            it += n;
         }
     } else {
         TLLM_PDL_WAIT();                                        // so are its scales
-        const int quad = warp & 3, half = (warp - 2) >> 2;      // a warp may read TMEM lanes 32 * (warp % 4) .. + 31
-        unsigned char* stage_out = tiles + (size_t)kStages * kStage + (size_t)(warp - 2) * 32 * kQPad;
+        const int quad = warp & 3, half = (warp - 3) >> 2;      // a warp may read TMEM lanes 32 * (warp % 4) .. + 31
+        unsigned char* stage_out = tiles + (size_t)kStages * kStage + (size_t)(warp - 3) * 32 * kQPad;
         int it = 0;
         for (int t = blockIdx.x; t < total; t += gridDim.x) {
             const int tile_m = t % p.tiles_m, rest = t / p.tiles_m, tile_n = rest % p.tiles_n, split = rest / p.tiles_n;
@@ -285,28 +304,30 @@ fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
             float acc[kCols];
 #pragma unroll
             for (int j = 0; j < kCols; ++j) acc[j] = 0.0f;
+            float s_x = sx[0], s_w = sw[0], s_u = INTER ? sw[p.kb_all] : 0.0f;
             bool ok = true;
             for (int kb = 0; kb < n; ++kb, ++it) {
                 const int buf = it % kBufs;
-                const float s0 = sx[kb];
-                const float s = s0 * sw[kb], s_up = INTER ? s0 * sw[p.kb_all + kb] : s;
-                ok = warp_wait(&part_full[buf], (it / kBufs) & 1, aborted, error_word, 3);
+                const uint64_t s = twice(s_x * s_w), s_up = INTER ? twice(s_x * s_u) : s;
+                if (kb + 1 < n) {
+                    s_x = sx[kb + 1];
+                    s_w = sw[kb + 1];
+                    if (INTER) s_u = sw[p.kb_all + kb + 1];
+                }
+                ok = quick_wait(&done_bar[it % kStages], (it / kStages) & 1, aborted, error_word, 3);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                 const uint32_t addr = tmem_base + buf * BN + half * kCols + ((uint32_t)(quad * 32) << 16);
+                uint32_t r[2][32];
+                tmem_ld32_issue(addr, r[0]);
+                tmem_ld32_issue(addr + 32, r[1]);
+                tmem_ld_wait();
+                asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&part_empty[buf]);
 #pragma unroll
-                for (int c = 0; c < kCols; c += 32) {
-                    uint32_t r[32];
-                    tmem_ld32_issue(addr + c, r);
-                    tmem_ld_wait();
-                    if (c + 32 >= kCols) {                       // all of this warp's numbers are in registers
-                        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&part_empty[buf]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) acc[c + j] = fmaf(__uint_as_float(r[j]), INTER && (j & 8) ? s_up : s, acc[c + j]);
-                }
+                for (int j = 0; j < kCols; j += 2)
+                    fma_pair(acc[j], acc[j + 1], r[j >> 5][j & 31], r[j >> 5][(j & 31) + 1], INTER && (j & 8) ? s_up : s);
             }
             if (!ok) break;
             finish_tile<OUT, kCols>(acc, p, stage_out, nullptr, row0, col0, tile_n, half, quad, lane, split, 0, aborted, error_word);
@@ -366,20 +387,6 @@ __device__ __forceinline__ void umma_commit_pair_if(uint32_t issue, uint64_t* ba
         "r"(issue), "h"((uint16_t)3)
         : "memory");
 }
-// Two sums at a time: (a, b) += (x, y) * (s, t).
-__device__ __forceinline__ void fma_pair(float& a, float& b, uint32_t x, uint32_t y, uint64_t st) {
-    uint64_t v, d;
-    asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "r"(x), "r"(y));
-    asm("mov.b64 %0, {%1, %2};\n" : "=l"(d) : "f"(a), "f"(b));
-    asm("fma.rn.f32x2 %0, %1, %2, %0;\n" : "+l"(d) : "l"(v), "l"(st));
-    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(d));
-}
-__device__ __forceinline__ uint64_t twice(float s) {
-    uint64_t d;
-    asm("mov.b64 %0, {%1, %1};\n" : "=l"(d) : "f"(s));
-    return d;
-}
-
 template <int OUT>
 __global__ void __launch_bounds__(kPairThreads, 1)
 fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Fp8Product p,
