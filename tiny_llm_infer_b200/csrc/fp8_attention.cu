@@ -6,33 +6,39 @@
 //
 //   out = sum_j 2^(s_j) sv_j v8_j / sum_j 2^(s_j).
 //
-// One block of threads owns (row, key/value head, run of keys): the query heads of the group are the rows of a 16-row tile, so a key and its
-// value come from HBM once per group: 2 hd + 8 bytes, half of the bfloat16 cache's.  What bounds it is their way from HBM.  Each of
-// the four warps walks every fourth tile of 16 keys: cp.async brings the tile's keys, values and scales into the warp's own ring; keys that do
-// not count (behind the row's position, before its window, without a page) arrive as zeros, so that what a page held before
-// meets no sum.
+// One block of threads owns (row, key/value head, run of keys): the query heads of the group share what is read, so a key and its value
+// come from HBM once per group: 2 hd + 8 bytes, half of the bfloat16 cache's.  What bounds it is their way from HBM.  The four warps take
+// units of 32 keys in turn: cp.async brings a unit's keys, values and scales into the warp's own ring of two while the unit before is
+// worked on; keys that do not count (behind the row's position, before its window, without a page) arrive as zeros, so that what a page
+// held before meets no sum.
 //
-// Products run on mma.sync m16n8k16 with float16 operands, which hold every e4m3 value exactly: queries are brought to float16 by a power
-// of two per head that puts the largest at 2^14 to 2^15, exact down to 2^-28 of the largest.  A lane's sixteen neighbouring
-// bytes of a key stand for the columns that four fragments assign to it, on the query's side alike, so keys need no rearrangement.  For
-// P V the fragments want two keys side by side: bytes of two keys are interleaved (prmt) before they become float16.
+// Products run on mma.sync m16n8k16 with float16 operands, which hold every e4m3 value exactly; keys and values are the left operands
+// (16 keys, or 16 dims, by 16) and eight query heads the right one, so a group of up to eight heads wastes nothing.  Queries are brought to
+// float16 by a power of two per head that puts the largest at 2^14 to 2^15, exact down to 2^-28 of the largest.  A lane's sixteen
+// neighbouring bytes of a key stand for the columns that four fragments assign to it, on the query's side alike, so keys need no
+// rearrangement.  For V^T P the fragments want two keys side by side: bytes of two keys are interleaved (prmt) before they become float16,
+// and the weights are turned by movmatrix.
 //
 // The softmax is online in float32 with two maxima: M of s_j for the denominator, and D of (s_j - M) + log2 sv_j for the weights
 // 2^((s_j - M) + log2 sv_j - D + 15) of the values, which are rounded to float16: relative to the heaviest term they keep 11 bits down to
 // 2^-29, whatever the values' scales, and what is lost below is under 2^-40 of it per key.  (D is relative to M, so that a score of any size
 // leaves the scale's logarithm its bits.)  The denominator sums unrounded numbers.
+//
+// With the heads as rows of a 16-row tile and 16 keys at a time a warp took 1.0 us a tile alone and 1.8 us beside eleven others (2.9 to
+// 3.9 TB/s): half of every product was wasted on missing rows, and the chain of scores, maxima and weights was walked twice as often.
 #include "fp8.cuh"
 #include "mma_tiles.cuh"
 
 namespace tllm {
 
-constexpr int kA8Warps = 4, kA8Keys = 16;
-constexpr int kA8Stages = 4;                     // tiles of a warp's ring: one in use, three on their way (12 KB of them at width 128)
+constexpr int kA8Warps = 4, kA8Unit = 32;        // keys a warp takes at a time
+constexpr int kA8Stages = 2;                     // units of a warp's ring: one in use, one on its way (8.4 KB at width 128)
 constexpr float kA8Lift = 15.0f;                 // weights are 2^15 at most
 
+// A unit in shared memory: keys, values, pairs of scales.
 template <int HD>
-struct A8Tile {
-    static constexpr int kPlane = kA8Keys * HD, kBytes = 2 * kPlane + kA8Keys * 8;
+struct A8Unit {
+    static constexpr int kPlane = kA8Unit * HD, kBytes = 2 * kPlane + kA8Unit * 8;
     // 16-byte chunk `chunk` of key `row`; both keep the reads of the main loop free of bank conflicts
     static __device__ __forceinline__ int key_at(int row, int chunk) { return HD == 128 ? row * 128 + ((chunk ^ ((row & 1) << 2)) << 4) : row * 64 + (chunk << 4); }
     static __device__ __forceinline__ int value_at(int row, int chunk) {
@@ -55,13 +61,32 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
     return *reinterpret_cast<uint32_t*>(&v);
 }
 
-__device__ __forceinline__ float quad_max(float v) {
-    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+// 2^x and log2 x by the special function unit (2 units in the last place; results below 2^-126 are zero).
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+// The largest (the sum) over the eight lanes that hold the same heads and other keys.
+__device__ __forceinline__ float keys_max(float v) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+__device__ __forceinline__ float keys_sum(float v) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// An 8 x 8 matrix of 16-bit numbers, a row in four lanes, turned.
+__device__ __forceinline__ uint32_t turned(uint32_t v) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(v));
+    return d;
 }
 
-// Runs of keys of one head added in order: sums and values of n runs, each with its M, D and l (`me` apart), one dim of its values (`oe`
-// apart).  M = max M_s, D = max (D_s + M_s - M); acc = sum o_s 2^(D_s + M_s - M - D), total = sum l_s 2^(M_s - M).  A run without keys has
+// The warps' runs of keys of one head added in order: sums and values of n runs, each with its M, D and l (`me` apart), one dim of its
+// values (`oe` apart).  M = max M_s, D = max (D_s + M_s - M); acc = sum o_s 2^(D_s + M_s - M - D), total = sum l_s 2^(M_s - M).  A run without keys has
 // M of -infinity and sums of zero; scores that are all NaN leave M so too, and l NaN.
 template <int UNROLL>
 __device__ __forceinline__ void join_runs(const float* m, int me, const float* o, int oe, int n, float& acc, float& total, float& mm, float& dn) {
@@ -85,15 +110,16 @@ __device__ __forceinline__ void join_runs(const float* m, int me, const float* o
     }
 }
 
-template <int HD>
-__global__ void __launch_bounds__(kA8Warps * 32, 3)
+// NT: eights of query heads per key/value head.
+template <int HD, int NT>
+__global__ void __launch_bounds__(kA8Warps * 32, NT == 1 ? 3 : 2)
 attention_fp8_decode_kernel(const bf16* q, const A8Cache cache, const int* __restrict__ positions, const int* __restrict__ token_slot,
                             const int* __restrict__ rows, const int* __restrict__ block_table, int max_pages, int page_size, int q_heads,
                             int kv_heads, int window, float scale_log2e, int splits, float* __restrict__ part_o,
                             float* __restrict__ part_m, bf16* __restrict__ out) {
     extern __shared__ __align__(128) unsigned char smem[];
     TLLM_PDL_ENTER();
-    using Tile = A8Tile<HD>;
+    using Unit = A8Unit<HD>;
     const int split = blockIdx.x, g = blockIdx.y, ridx = blockIdx.z;
     const int r = rows ? rows[ridx] : ridx;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3, gr = lane >> 2;
@@ -106,44 +132,62 @@ attention_fp8_decode_kernel(const bf16* q, const A8Cache cache, const int* __res
     }
     const int pos = positions[r];
     const int lo = (window > 0 && pos - window + 1 > 0) ? pos - window + 1 : 0;
-    const int base = lo / kA8Keys * kA8Keys;
-    const int tiles_all = (pos - base) / kA8Keys + 1;
-    int per = (tiles_all + splits - 1) / splits;
+    const int base = lo / 16 * 16;                                 // 16 keys never straddle a page
+    const int units_all = (pos - base) / kA8Unit + 1;
+    int per = (units_all + splits - 1) / splits;
     per = (per + kA8Warps - 1) / kA8Warps * kA8Warps;              // whole rounds of the four warps
-    const int tile0 = base / kA8Keys + split * per;
-    const int tile_end = min(base / kA8Keys + tiles_all, tile0 + per);
+    const int unit_end = min(units_all, split * per + per);
+    int unit = split * per + warp;
     const int* table = block_table + (size_t)slot * max_pages;
-    unsigned char* ring = smem + (size_t)warp * kA8Stages * Tile::kBytes;
+    unsigned char* ring = smem + (size_t)warp * kA8Stages * Unit::kBytes;
 
-    auto issue = [&](int tile, int stage) {
-        if (tile < tile_end) {
-            const int key0 = tile * kA8Keys;
-            const int page = table[key0 / page_size];
-            const size_t at = (size_t)max(page, 0) * cache.stride, token0 = (size_t)g * page_size + key0 % page_size;
-            const uint8_t *kp = cache.k + at + token0 * HD, *vp = cache.v + at + token0 * HD, *sp = cache.scales + at + token0 * 8;
-            const uint32_t ks = smem_u32(ring + (size_t)stage * Tile::kBytes), vs = ks + Tile::kPlane, ss = vs + Tile::kPlane;
-            const bool whole = page >= 0 && key0 >= lo && key0 + kA8Keys - 1 <= pos;
+    // ---- the next unit to fetch: its first key, that key's page (index in the table) and place in it, for both of its sixteens
+    int f_unit = unit, f_stage = 0, key0 = base + unit * kA8Unit;
+    int page_at = key0 / page_size, in_page = key0 - page_at * page_size;
+    constexpr int kStep = kA8Warps * kA8Unit;
+    const int step_pages = kStep / page_size, step_rest = kStep - step_pages * page_size;
+    const uint8_t* const k0 = cache.k + lane * 16;
+    const uint8_t* const v0 = cache.v + lane * 16;
+    const int key_dst = Unit::key_at(lane / (HD / 16), lane % (HD / 16));
+    auto fetch = [&]() {
+        if (f_unit < unit_end) {
+            const bool wraps = in_page + 16 >= page_size;
+            const uint32_t dst = smem_u32(ring + (size_t)f_stage * Unit::kBytes);
 #pragma unroll
-            for (int i = 0; i < Tile::kPlane / 16 / 32; ++i) {
-                const int n = lane + 32 * i, row = n / (HD / 16), chunk = n % (HD / 16);
-                const bool ok = whole || (page >= 0 && key0 + row >= lo && key0 + row <= pos);
-                cp_async_16(ks + Tile::key_at(row, chunk), kp + n * 16, ok);
-                cp_async_16(vs + Tile::value_at(row, chunk), vp + n * 16, ok);
+            for (int h = 0; h < 2; ++h) {
+                const int first = key0 + 16 * h;
+                const int page = first <= pos ? table[h && wraps ? page_at + 1 : page_at] : -1;
+                const size_t at = (size_t)max(page, 0) * cache.stride, token = (size_t)g * page_size + (h == 0 ? in_page : wraps ? in_page + 16 - page_size : in_page + 16);
+                const uint8_t *kp = k0 + at + token * HD, *vp = v0 + at + token * HD;
+                const bool whole = page >= 0 && first >= lo && first + 15 <= pos;
+                constexpr int kPieces = 16 * HD / 16 / 32;         // per lane: 4 or 2
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    const int n = lane + 32 * i, row = n / (HD / 16), chunk = n % (HD / 16);
+                    const bool ok = whole || (page >= 0 && first + row >= lo && first + row <= pos);
+                    cp_async_16(dst + key_dst + h * 16 * HD + i * 512, kp + i * 512, ok);
+                    cp_async_16(dst + Unit::kPlane + Unit::value_at(row, chunk) + h * 16 * HD, vp + i * 512, ok);
+                }
+                if (lane < 8) cp_async_16(dst + 2 * Unit::kPlane + h * 128 + lane * 16, cache.scales + at + token * 8 + lane * 16, page >= 0);   // masked below
             }
-            if (lane < 8) cp_async_16(ss + lane * 16, sp + lane * 16, page >= 0);       // two keys' scales: masked below
+            f_unit += kA8Warps;
+            key0 += kStep;
+            page_at += step_pages;
+            in_page += step_rest;
+            if (in_page >= page_size) in_page -= page_size, ++page_at;
+            f_stage = f_stage + 1 == kA8Stages ? 0 : f_stage + 1;
         }
         cp_async_commit();                                         // one group per call, empty past the end
     };
-    int tile = tile0 + warp;
 #pragma unroll
-    for (int st = 0; st < kA8Stages - 1; ++st) issue(tile + st * kA8Warps, st);
+    for (int st = 0; st < kA8Stages - 1; ++st) fetch();
 
-    // queries in float16, each head times a power of two; fragment (h, w) has dims 64 h + 16 c + 4 w .. + 3 of this lane
-    uint32_t qa[HD / 16][4];
-    float to_score[2];                                             // of heads gr and gr + 8: what turns a product into s
+    // ---- queries in float16, each head times a power of two; fragment (h, i) has dims 64 h + 16 c + 4 i .. + 3 of head nt * 8 + gr
+    uint32_t qb[NT][HD / 16][2];
+    float to_score[NT][2];                                         // of heads nt * 8 + 2 c, + 1: what turns a product into s
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const int head = gr + 8 * half;
+    for (int nt = 0; nt < NT; ++nt) {
+        const int head = nt * 8 + gr;
         const bf16* qp = q + ((size_t)r * q_heads + (size_t)g * group + min(head, group - 1)) * HD;
         float v[HD / 4];
         float largest = 0.0f;
@@ -160,155 +204,184 @@ attention_fp8_decode_kernel(const bf16* q, const A8Cache cache, const int* __res
                     largest = fmaxf(largest, fmaxf(fabsf(low_float(p[j])), fabsf(high_float(p[j]))));
                 }
             }
-        largest = quad_max(largest);
+        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
         // 2^(14 - exponent): as a product of two factors, each within float32's range for every bfloat16
         const int e = (__float_as_int(largest) >> 23) & 255;       // biased exponent; 0 for zeros and the smallest, 255 for infinities
         const int shift = e == 255 ? 0 : 14 + 127 - max(e, 1);     // -113 .. 140
         const float f0 = __int_as_float((127 + shift / 2) << 23), f1 = __int_as_float((127 + shift - shift / 2) << 23);
         const float b0 = __int_as_float((127 - shift / 2) << 23), b1 = __int_as_float((127 - (shift - shift / 2)) << 23);
-        to_score[half] = scale_log2e * b0 * b1;
+        const float back = scale_log2e * b0 * b1;
+        const bool live = head < group;
 #pragma unroll
         for (int f = 0; f < HD / 16; ++f) {
             const float* x = v + 4 * f;
-            const bool live = head < group;
-            qa[f][half] = live ? pack_half(x[0] * f0 * f1, x[1] * f0 * f1) : 0u;
-            qa[f][2 + half] = live ? pack_half(x[2] * f0 * f1, x[3] * f0 * f1) : 0u;
+            qb[nt][f][0] = live ? pack_half(x[0] * f0 * f1, x[1] * f0 * f1) : 0u;
+            qb[nt][f][1] = live ? pack_half(x[2] * f0 * f1, x[3] * f0 * f1) : 0u;
         }
+#pragma unroll
+        for (int e2 = 0; e2 < 2; ++e2) to_score[nt][e2] = __shfl_sync(0xffffffffu, back, (2 * c + e2) * 4);
     }
 
-    float o[HD / 8][4];                                            // o[i]: dims gr' (HD / 8) + i of columns gr' = 2 c, 2 c + 1
+    constexpr int kMT = HD / 16;                                   // tiles of 16 dims; of a lane the dims gr (HD / 8) + 2 t, + 1 are rows gr, gr + 8 of tile t
+    float o[NT][kMT][4];
+    float m[NT][2], dd[NT][2], l[NT][2];                           // of heads nt * 8 + 2 c, + 1: M, D, sum over this lane's keys
 #pragma unroll
-    for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, dd[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};   // M, D, sum
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int t = 0; t < kMT; ++t) o[nt][t][0] = o[nt][t][1] = o[nt][t][2] = o[nt][t][3] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) m[nt][e] = dd[nt][e] = -INFINITY, l[nt][e] = 0.0f;
+    }
 
-    for (int stage = 0; tile < tile_end; tile += kA8Warps, stage = (stage + 1) % kA8Stages) {
+    for (int stage = 0; unit < unit_end; unit += kA8Warps, stage = stage + 1 == kA8Stages ? 0 : stage + 1) {
         __syncwarp();                                              // the stage refilled below has been read by all lanes
-        issue(tile + (kA8Stages - 1) * kA8Warps, (stage + kA8Stages - 1) % kA8Stages);
+        fetch();
         cp_async_wait<kA8Stages - 1>();
         __syncwarp();
-        const unsigned char *kt = ring + (size_t)stage * Tile::kBytes, *vt = kt + Tile::kPlane;
-        const float* st = reinterpret_cast<const float*>(vt + Tile::kPlane);
+        const unsigned char *kt = ring + (size_t)stage * Unit::kBytes, *vt = kt + Unit::kPlane;
+        const float2* st = reinterpret_cast<const float2*>(vt + Unit::kPlane);
 
-        float s[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        // ---- scores: s[nt][h][e], s[nt][h][2 + e]: keys 16 h + gr and 16 h + gr + 8, head nt * 8 + 2 c + e
+        float s[NT][2][4];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int h = 0; h < HD / 64; ++h) {
-                const uint4 raw = *reinterpret_cast<const uint4*>(kt + Tile::key_at(nt * 8 + gr, 4 * h + c));
-                const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+            for (int h = 0; h < 2; ++h) s[nt][h][0] = s[nt][h][1] = s[nt][h][2] = s[nt][h][3] = 0.0f;
+#pragma unroll
+        for (int f = 0; f < HD / 64; ++f)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint4 ra = *reinterpret_cast<const uint4*>(kt + Unit::key_at(16 * h + gr, 4 * f + c));
+                const uint4 rb = *reinterpret_cast<const uint4*>(kt + Unit::key_at(16 * h + gr + 8, 4 * f + c));
+                const uint32_t wa[4] = {ra.x, ra.y, ra.z, ra.w}, wb[4] = {rb.x, rb.y, rb.z, rb.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t b[2] = {e4m3x2_to_half2(w[i]), e4m3x2_to_half2(w[i] >> 16)};
-                    mma_f16_16816(s[nt], qa[4 * h + i], b);
+                    const uint32_t a[4] = {e4m3x2_to_half2(wa[i]), e4m3x2_to_half2(wb[i]), e4m3x2_to_half2(wa[i] >> 16), e4m3x2_to_half2(wb[i] >> 16)};
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_f16_16816(s[nt][h], a, qb[nt][4 * f + i]);
                 }
             }
-        // s[nt][e], s[nt][2 + e]: heads gr and gr + 8, key nt * 8 + 2 c + e
-        float lv[2][2], tm[2] = {-INFINITY, -INFINITY};
+        const int first = base + unit * kA8Unit + gr;
+        const bool whole = base + unit * kA8Unit >= lo && base + unit * kA8Unit + kA8Unit - 1 <= pos;
+        float lv[2][2];                                            // log2 of the values' scales, keys 16 h + gr + 8 e
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-            const float4 sc = *reinterpret_cast<const float4*>(st + (nt * 8 + 2 * c) * 2);
-            const int j = tile * kA8Keys + nt * 8 + 2 * c;
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const bool ok = j + e >= lo && j + e <= pos;
-                const float sk = e ? sc.z : sc.x;
-                lv[nt][e] = ok ? __log2f(e ? sc.w : sc.y) : -INFINITY;
+                const float2 sc = st[16 * h + 8 * e + gr];
+                const int j = first + 16 * h + 8 * e;
+                const bool ok = whole || (j >= lo && j <= pos);
+                lv[h][e] = ok ? __log2f(sc.y) : -INFINITY;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    float& x = s[nt][2 * half + e];
-                    x = ok ? x * (sk * to_score[half]) : -INFINITY;
-                    tm[half] = fmaxf(tm[half], x);
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        float& x = s[nt][h][2 * e + n];
+                        x = ok ? x * (sc.x * to_score[nt][n]) : -INFINITY;
+                    }
+            }
+        // ---- maxima, sums and weights, head by head
+        uint32_t pb[NT][2][2];                                     // weights as the right operand: keys 2 c, + 1 (and 8 further) of sixteen h, head gr
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float w[2][4], cu[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const float mn = fmaxf(m[nt][n], keys_max(fmaxf(fmaxf(s[nt][0][n], s[nt][0][2 + n]), fmaxf(s[nt][1][n], s[nt][1][2 + n]))));
+                const float ms = mn == -INFINITY ? 0.0f : mn, back = m[nt][n] - ms;        // -infinity before the first key
+                float sum = 0.0f, td = -INFINITY;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float t = s[nt][h][2 * e + n] - ms;
+                        sum += fast_exp2(t);
+                        w[h][2 * e + n] = t + lv[h][e];
+                        td = fmaxf(td, w[h][2 * e + n]);
+                    }
+                const float dn = fmaxf(dd[nt][n] + back, keys_max(td)), ds = dn == -INFINITY ? 0.0f : dn;
+                cu[n] = fast_exp2(dd[nt][n] + back - ds);
+                l[nt][n] = l[nt][n] * fast_exp2(back) + sum;
+                m[nt][n] = mn;
+                dd[nt][n] = dn;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) w[h][2 * e + n] = fast_exp2(w[h][2 * e + n] - ds + kA8Lift);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) pb[nt][h][e] = turned(pack_half(w[h][2 * e], w[h][2 * e + 1]));
+            if (__any_sync(0xffffffffu, cu[0] != 1.0f || cu[1] != 1.0f)) {                 // seldom after the first units
+#pragma unroll
+                for (int t = 0; t < kMT; ++t) {
+                    o[nt][t][0] *= cu[0];
+                    o[nt][t][1] *= cu[1];
+                    o[nt][t][2] *= cu[0];
+                    o[nt][t][3] *= cu[1];
                 }
             }
         }
-        float w[2][4];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const float mn = fmaxf(m[half], quad_max(tm[half]));
-            const float ms = mn == -INFINITY ? 0.0f : mn, back = m[half] - ms;      // -infinity before the first key
-            float sum = 0.0f, td = -INFINITY;
-#pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float t = s[nt][2 * half + e] - ms;
-                    sum += exp2f(t);
-                    w[nt][2 * half + e] = t + lv[nt][e];
-                    td = fmaxf(td, w[nt][2 * half + e]);
-                }
-            const float dn = fmaxf(dd[half] + back, quad_max(td)), ds = dn == -INFINITY ? 0.0f : dn;
-            const float cu = exp2f(dd[half] + back - ds);
-            l[half] = l[half] * exp2f(back) + sum;
-            m[half] = mn;
-            dd[half] = dn;
-#pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) w[nt][2 * half + e] = exp2f(w[nt][2 * half + e] - ds + kA8Lift);
-#pragma unroll
-            for (int i = 0; i < HD / 8; ++i) {
-                o[i][2 * half] *= cu;
-                o[i][2 * half + 1] *= cu;
-            }
-        }
-        const uint32_t pa[4] = {pack_half(w[0][0], w[0][1]), pack_half(w[0][2], w[0][3]), pack_half(w[1][0], w[1][1]), pack_half(w[1][2], w[1][3])};
-        // values of keys 2 c, 2 c + 1 and eight further, dims gr (HD / 8) .. + HD / 8 - 1
+        // ---- values of keys 2 c, 2 c + 1 and eight further of each sixteen, dims gr (HD / 8) .. + HD / 8 - 1
         constexpr int kWords = HD / 32;
-        uint32_t vw[4][kWords];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = 2 * c + (i & 1) + (i >> 1) * 8;
-            if constexpr (HD == 128) {
-                const uint4 raw = *reinterpret_cast<const uint4*>(vt + Tile::value_at(row, gr));
-                vw[i][0] = raw.x; vw[i][1] = raw.y; vw[i][2] = raw.z; vw[i][3] = raw.w;
-            } else {
-                const uint2 raw = *reinterpret_cast<const uint2*>(vt + Tile::value_at(row, gr >> 1) + (gr & 1) * 8);
-                vw[i][0] = raw.x; vw[i][1] = raw.y;
+        for (int h = 0; h < 2; ++h) {
+            uint32_t vw[4][kWords];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = 16 * h + 2 * c + (i & 1) + (i >> 1) * 8;
+                if constexpr (HD == 128) {
+                    const uint4 raw = *reinterpret_cast<const uint4*>(vt + Unit::value_at(row, gr));
+                    vw[i][0] = raw.x; vw[i][1] = raw.y; vw[i][2] = raw.z; vw[i][3] = raw.w;
+                } else {
+                    const uint2 raw = *reinterpret_cast<const uint2*>(vt + Unit::value_at(row, gr >> 1) + (gr & 1) * 8);
+                    vw[i][0] = raw.x; vw[i][1] = raw.y;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                const uint32_t x0 = pairs_low(vw[0][i], vw[1][i]), x1 = pairs_high(vw[0][i], vw[1][i]);
+                const uint32_t y0 = pairs_low(vw[2][i], vw[3][i]), y1 = pairs_high(vw[2][i], vw[3][i]);
+                const uint32_t a0[4] = {e4m3x2_to_half2(x0), e4m3x2_to_half2(x0 >> 16), e4m3x2_to_half2(y0), e4m3x2_to_half2(y0 >> 16)};
+                const uint32_t a1[4] = {e4m3x2_to_half2(x1), e4m3x2_to_half2(x1 >> 16), e4m3x2_to_half2(y1), e4m3x2_to_half2(y1 >> 16)};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma_f16_16816(o[nt][2 * i], a0, pb[nt][h]);
+                    mma_f16_16816(o[nt][2 * i + 1], a1, pb[nt][h]);
+                }
             }
         }
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-            const uint32_t a0 = pairs_low(vw[0][i], vw[1][i]), a1 = pairs_high(vw[0][i], vw[1][i]);
-            const uint32_t b0 = pairs_low(vw[2][i], vw[3][i]), b1 = pairs_high(vw[2][i], vw[3][i]);
-            const uint32_t d[4][2] = {{e4m3x2_to_half2(a0), e4m3x2_to_half2(b0)}, {e4m3x2_to_half2(a0 >> 16), e4m3x2_to_half2(b0 >> 16)},
-                                      {e4m3x2_to_half2(a1), e4m3x2_to_half2(b1)}, {e4m3x2_to_half2(a1 >> 16), e4m3x2_to_half2(b1 >> 16)}};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mma_f16_16816(o[4 * i + e], pa, d[e]);
-        }
-    }
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
-        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
     }
     // ---- the four warps' results are added in shared memory, which the ring no longer needs
     cp_async_wait<0>();
     __syncthreads();
-    float* os = reinterpret_cast<float*>(smem);                    // [warps][16][HD]
-    float* ms = os + kA8Warps * 16 * HD;                           // [warps][16][3]: M, D, L
+    float* os = reinterpret_cast<float*>(smem);                    // [warps][8 NT][HD]
+    float* ms = os + kA8Warps * 8 * NT * HD;                       // [warps][8 NT][3]: M, D, sum
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const int row = gr + 8 * half;
-        if (row < group) {
-            float* dst = os + ((size_t)warp * 16 + row) * HD;
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+        for (int n = 0; n < 2; ++n) {
+            const int row = nt * 8 + 2 * c + n;
+            const float sum = keys_sum(l[nt][n]);
+            if (row < group) {
+                float* dst = os + ((size_t)warp * 8 * NT + row) * HD + gr * (HD / 8);
 #pragma unroll
-                for (int i = 0; i < HD / 8; i += 4)
-                    *reinterpret_cast<float4*>(dst + (2 * c + e) * (HD / 8) + i) =
-                        make_float4(o[i][2 * half + e], o[i + 1][2 * half + e], o[i + 2][2 * half + e], o[i + 3][2 * half + e]);
-            if (c == 0) {
-                ms[(warp * 16 + row) * 3] = m[half];
-                ms[(warp * 16 + row) * 3 + 1] = dd[half];
-                ms[(warp * 16 + row) * 3 + 2] = l[half];
+                for (int t = 0; t < kMT; t += 2)
+                    *reinterpret_cast<float4*>(dst + 2 * t) = make_float4(o[nt][t][n], o[nt][t][2 + n], o[nt][t + 1][n], o[nt][t + 1][2 + n]);
+                if (gr == 0) {
+                    ms[(warp * 8 * NT + row) * 3] = m[nt][n];
+                    ms[(warp * 8 * NT + row) * 3 + 1] = dd[nt][n];
+                    ms[(warp * 8 * NT + row) * 3 + 2] = sum;
+                }
             }
         }
-    }
     __syncthreads();
     for (int idx = threadIdx.x; idx < group * HD; idx += blockDim.x) {
         const int row = idx / HD, d = idx - row * HD;
         float acc, total, mm, dn;
-        join_runs<kA8Warps>(ms + row * 3, 16 * 3, os + (size_t)row * HD + d, 16 * HD, kA8Warps, acc, total, mm, dn);
+        join_runs<kA8Warps>(ms + row * 3, 8 * NT * 3, os + (size_t)row * HD + d, 8 * NT * HD, kA8Warps, acc, total, mm, dn);
         const int head = g * group + row;
         if (splits == 1) {
             const float up = dn == -INFINITY ? 0.0f : exp2f(dn - kA8Lift);
@@ -321,39 +394,82 @@ attention_fp8_decode_kernel(const bf16* q, const A8Cache cache, const int* __res
     }
 }
 
+// The runs of a (row, head) added.  Every warp finds the runs' factors, a lane each for every 32nd run; then the block's kA8JoinGroups groups of HD
+// threads add every kA8JoinGroups-th run's values, eight of them on their way at once, and the groups' sums are added in order.  (One thread per dim
+// that walked over 64 runs one by one took 43 us.)
+constexpr int kA8JoinGroups = 4, kA8MaxRuns = 128;
 template <int HD>
-__global__ void attention_fp8_join_kernel(const float* part_o, const float* part_m, const int* __restrict__ token_slot,
-                                          const int* __restrict__ rows, int q_heads, int splits, bf16* __restrict__ out) {
+__global__ void __launch_bounds__(HD * kA8JoinGroups)
+attention_fp8_join_kernel(const float* part_o, const float* part_m, const int* __restrict__ token_slot, const int* __restrict__ rows, int q_heads,
+                          int splits, bf16* __restrict__ out) {
+    __shared__ float factor[kA8MaxRuns], sums[kA8JoinGroups][HD];
     TLLM_PDL_ENTER();
-    const int ridx = blockIdx.x, head = blockIdx.y, d = threadIdx.x;
+    const int ridx = blockIdx.x, head = blockIdx.y, d = threadIdx.x % HD, group = threadIdx.x / HD, lane = threadIdx.x & 31;
     const int r = rows ? rows[ridx] : ridx;
     bf16* dst = out + ((size_t)r * q_heads + head) * HD;
-    if (token_slot[r] < 0) { dst[d] = __float2bfloat16_rn(0.0f); return; }
+    if (token_slot[r] < 0) {
+        if (group == 0) dst[d] = __float2bfloat16_rn(0.0f);
+        return;
+    }
     const size_t base = ((size_t)ridx * q_heads + head) * splits;
-    float acc, total, mm, dn;
-    join_runs<1>(part_m + base * 3, 3, part_o + base * HD + d, HD, splits, acc, total, mm, dn);
+    constexpr int kEach = kA8MaxRuns / 32;
+    float m[kEach], dd[kEach], l[kEach], mm = -INFINITY, dn = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int s = lane + 32 * i;
+        const float* e = part_m + (base + s) * 3;
+        const bool there = s < splits;
+        m[i] = there ? e[0] : -INFINITY;
+        dd[i] = there ? e[1] : -INFINITY;
+        l[i] = there ? e[2] : 0.0f;
+        mm = fmaxf(mm, m[i]);
+    }
+    mm = warp_max(mm);
+    // a run without keys has M of -infinity and sums of zero; scores that are all NaN leave M so too, and l NaN
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        dd[i] = m[i] == -INFINITY ? -INFINITY : dd[i] + (m[i] - mm);
+        total += m[i] == -INFINITY ? l[i] : l[i] * exp2f(m[i] - mm);
+        dn = fmaxf(dn, dd[i]);
+    }
+    dn = warp_max(dn);
+    total = warp_sum(total);
+    if (threadIdx.x < 32)
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (lane + 32 * i < splits) factor[lane + 32 * i] = dd[i] == -INFINITY ? 0.0f : exp2f(dd[i] - dn);
+    __syncthreads();
+    float acc = 0.0f;
+    const float* o = part_o + base * HD + d;
+#pragma unroll 8
+    for (int s = group; s < splits; s += kA8JoinGroups) acc = fmaf(o[(size_t)s * HD], factor[s], acc);
+    sums[group][d] = acc;
+    __syncthreads();
+    if (group != 0) return;
+#pragma unroll
+    for (int g = 1; g < kA8JoinGroups; ++g) acc += sums[g][d];
     const float up = dn == -INFINITY ? 0.0f : exp2f(dn - kA8Lift);
     dst[d] = __float2bfloat16_rn(acc * up / total);
 }
 
-template <int HD>
+template <int HD, int NT>
 static int launch_attention_fp8(const void* q, const A8Cache& cache, const int* positions, const int* token_slot, const int* rows, int n_rows,
                                 const int* block_table, int max_pages, int page_size, int q_heads, int kv_heads, int window, float scale,
                                 int splits, float* part_o, float* part_m, void* out, cudaStream_t stream) {
-    constexpr size_t ring = (size_t)kA8Warps * kA8Stages * A8Tile<HD>::kBytes, joined = (size_t)kA8Warps * 16 * (HD + 3) * sizeof(float);
+    constexpr size_t ring = (size_t)kA8Warps * kA8Stages * A8Unit<HD>::kBytes, joined = (size_t)kA8Warps * 8 * NT * (HD + 3) * sizeof(float);
     constexpr size_t smem = ring > joined ? ring : joined;
     static OncePerDevice configured;
     if (configured.first()) {
-        cudaError_t e = cudaFuncSetAttribute(attention_fp8_decode_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        cudaError_t e = cudaFuncSetAttribute(attention_fp8_decode_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) { set_error("attention_fp8_decode: %s", cudaGetErrorString(e)); return (int)e; }
         configured.done();
     }
-    launch_pdl(kPdlAttention, attention_fp8_decode_kernel<HD>, dim3(splits, kv_heads, n_rows), dim3(kA8Warps * 32), smem, stream,
+    launch_pdl(kPdlAlways, attention_fp8_decode_kernel<HD, NT>, dim3(splits, kv_heads, n_rows), dim3(kA8Warps * 32), smem, stream,
                (const bf16*)q, cache, positions, token_slot, rows, block_table, max_pages, page_size, q_heads, kv_heads, window,
                scale * 1.4426950408889634f, splits, part_o, part_m, (bf16*)out);
     const int rc = finish_launch("attention_fp8_decode");
     if (rc != 0 || splits == 1) return rc;
-    launch_pdl(kPdlCombine, attention_fp8_join_kernel<HD>, dim3(n_rows, q_heads), dim3(HD), 0, stream, (const float*)part_o, (const float*)part_m,
+    launch_pdl(kPdlAlways, attention_fp8_join_kernel<HD>, dim3(n_rows, q_heads), dim3(HD * kA8JoinGroups), 0, stream, (const float*)part_o, (const float*)part_m,
                token_slot, rows, q_heads, splits, (bf16*)out);
     return finish_launch("attention_fp8_join");
 }
@@ -433,16 +549,23 @@ extern "C" int tllm_attention_fp8_decode(const void* q, const void* k, const voi
     if (check_a8("attention_fp8_decode", k, v, scales, page_bytes, page_size, kv_heads, head_dim) != 0) return -1;
     TLLM_REQUIRE(q_heads > 0 && q_heads % kv_heads == 0 && q_heads / kv_heads <= 16,
                  "attention_fp8_decode: %d query heads over %d key/value heads (at most 16 per group)", q_heads, kv_heads);
-    TLLM_REQUIRE(splits >= 1 && splits <= 65535 && n_rows >= 0 && n_rows <= 65535 && q_heads <= 65535 && max_pages > 0, "attention_fp8_decode: bad grid");
+    TLLM_REQUIRE(splits >= 1 && splits <= kA8MaxRuns && n_rows >= 0 && n_rows <= 65535 && q_heads <= 65535 && max_pages > 0, "attention_fp8_decode: bad grid");
     TLLM_REQUIRE(splits == 1 || (part_o && part_m), "attention_fp8_decode: %d runs of keys need scratch", splits);
     TLLM_REQUIRE(q && out && positions && token_slot && block_table && (reinterpret_cast<uintptr_t>(q) & 15u) == 0,
                  "attention_fp8_decode: missing or unaligned operands");
     if (n_rows == 0) return 0;
     const A8Cache cache{(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)scales, page_bytes};
-    return head_dim == 64 ? launch_attention_fp8<64>(q, cache, positions, token_slot, rows, n_rows, block_table, max_pages, page_size, q_heads, kv_heads,
-                                                     window, scale, splits, part_o, part_m, out, stream)
-                          : launch_attention_fp8<128>(q, cache, positions, token_slot, rows, n_rows, block_table, max_pages, page_size, q_heads, kv_heads,
-                                                      window, scale, splits, part_o, part_m, out, stream);
+#define ATTEND(HD, NT)                                                                                                                       \
+    return launch_attention_fp8<HD, NT>(q, cache, positions, token_slot, rows, n_rows, block_table, max_pages, page_size, q_heads, kv_heads, \
+                                        window, scale, splits, part_o, part_m, out, stream)
+    const bool one = q_heads / kv_heads <= 8;
+    if (head_dim == 64) {
+        if (one) ATTEND(64, 1);
+        ATTEND(64, 2);
+    }
+    if (one) ATTEND(128, 1);
+    ATTEND(128, 2);
+#undef ATTEND
 }
 
 // seg_info [segments][4] = slot, first row, tokens, position of the first.  `per`: pages of the portion that has most; pages bfloat16
@@ -456,10 +579,10 @@ extern "C" int tllm_attention_fp8_unpack(const void* k, const void* v, const voi
     TLLM_REQUIRE((long long)2 * kv_heads * page_size * (head_dim / 16) <= 0x7fffffff, "attention_fp8_unpack: too large");
     const A8Cache cache{(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)scales, page_bytes};
     if (head_dim == 64)
-        launch_pdl(kPdlOther, attention_fp8_unpack_kernel<64>, dim3(per, segments), dim3(256), 0, stream, cache, seg_info, block_table, max_pages,
+        launch_pdl(kPdlAlways, attention_fp8_unpack_kernel<64>, dim3(per, segments), dim3(256), 0, stream, cache, seg_info, block_table, max_pages,
                    page_size, kv_heads, window, capacity, (bf16*)pages, table);
     else
-        launch_pdl(kPdlOther, attention_fp8_unpack_kernel<128>, dim3(per, segments), dim3(256), 0, stream, cache, seg_info, block_table, max_pages,
+        launch_pdl(kPdlAlways, attention_fp8_unpack_kernel<128>, dim3(per, segments), dim3(256), 0, stream, cache, seg_info, block_table, max_pages,
                    page_size, kv_heads, window, capacity, (bf16*)pages, table);
     return finish_launch("attention_fp8_unpack");
 }
