@@ -40,9 +40,9 @@ def test_values_follow_the_layout_of_the_scales():
 @pytest.mark.parametrize("rows", [33, 64, 128, 129, 500, 2048, 100000])
 @pytest.mark.parametrize("n,k", [(8, 16), (1024, 128), (4096, 4096), (24576, 4096), (130, 12288)])
 def test_shares_cover_all_blocks_and_none_is_empty(rows, n, k):
-    pairs, splits, each = fp8._plan(rows, n, k, 148)
+    route, splits, each = fp8._plan(rows, n, k, 148)
     kb = -(-k // 128)
-    assert (splits == 1 or not pairs) and (splits - 1) * each < kb <= splits * each
+    assert (splits == 1 or route == fp8.TILES) and (splits - 1) * each < kb <= splits * each
 
 
 def test_tensors_of_the_host_are_refused():

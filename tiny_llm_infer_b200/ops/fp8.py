@@ -13,6 +13,7 @@ Infinities and NaN in a row of x reach the outputs of that row alone (as NaN), i
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -23,9 +24,16 @@ SMALLEST = 2.0 ** -100
 LARGEST = 448.0
 
 
+_package = None
+
+
 def _ops():
-    from .. import ops
-    return ops
+    """The package of the kernels (imported late: it imports this module)."""
+    global _package
+    if _package is None:
+        from .. import ops
+        _package = ops
+    return _package
 
 
 def declare(h) -> None:
@@ -33,12 +41,10 @@ def declare(h) -> None:
     vp, i32, f32, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
     sigs = {
         "tllm_fp8_rows": [vp, i32, vp, vp, i32, i32, vp],
-        "tllm_fp8_gated_rows": [vp, i32, vp, vp, i32, i32, i32, f32, f32, vp],
+        "tllm_fp8_linear": [vp, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp],
+        "tllm_fp8_gated": [vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, f32, vp, vp, vp],
         "tllm_add_rmsnorm_fp8": [vp, vp, i32, vp, i32, f32, vp, vp, i32, i32, vp],
         "tllm_fp8_weight": [vp, i32, vp, vp, i32, i32, i32, vp],
-        "tllm_fp8_skinny": [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, f32, f32, vp],
-        "tllm_fp8_tcgen05": [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, f32, f32, vp, vp],
-        "tllm_fp8_join": [vp, i32, i64, vp, i32, vp],
         "tllm_qk_norm_rope_store_fp8": [vp, vp, vp, i32, f32, vp, i32, vp, vp, vp, i32, vp, vp, vp, i64, i32, vp, i32, i32, i32, i32, i32,
                                         vp, vp],
         "tllm_attention_fp8_decode": [vp, vp, vp, vp, i64, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, f32, i32, vp, vp, vp, vp],
@@ -60,15 +66,15 @@ def _refuse(text: str):
 
 def _here(*tensors) -> None:
     """Contiguous CUDA tensors of the current device (the kernels go to its current stream)."""
-    current = None
+    current = -2
     for t in tensors:
         if t is None:
             continue
         if not t.is_cuda or not t.is_contiguous():
             _refuse("kernels take contiguous CUDA tensors")
-        if current is None:
-            current = torch.cuda.current_device()
-        if t.device.index != current:
+        if current == -2:
+            current = _ops()._raw_device()
+        if t.get_device() != current:
             _refuse(f"a tensor of {t.device}, the current device is cuda:{current}")
 
 
@@ -76,7 +82,7 @@ class Fp8Weight:
     """A weight [N, K] as e4m3 values ``q`` and float32 ``scales`` [ceil(N / 128), ceil(K / 128)].  ``gated``: the rows are N / 2 gate
     and N / 2 up rows interleaved by eight (``ops.interleave_gate_up``), and the scales [2 ceil(N / 2 / 128), ceil(K / 128)] are those
     of 128 gate rows, of the up rows that belong to them, and so on.  K is a multiple of 16."""
-    __slots__ = ("q", "scales", "gated")
+    __slots__ = ("q", "scales", "gated", "shape", "pointers", "index")
 
     def __init__(self, q: torch.Tensor, scales: torch.Tensor, gated: bool = False):
         if q.dtype != E4M3 or q.dim() != 2 or scales.dtype != torch.float32:
@@ -92,10 +98,8 @@ class Fp8Weight:
         if q.device != scales.device or not q.is_contiguous() or not scales.is_contiguous() or q.data_ptr() % 16:
             _refuse("an 8-bit weight and its scales are contiguous on one device, the weight 16-byte aligned")
         self.q, self.scales, self.gated = q, scales, bool(gated)
-
-    @property
-    def shape(self):
-        return self.q.shape
+        # what every product asks for: the weight keeps its tensors, so their addresses are its own
+        self.shape, self.pointers, self.index = q.shape, (q.data_ptr(), scales.data_ptr()), q.get_device()
 
     @property
     def dtype(self):
@@ -118,8 +122,9 @@ class Fp8Weight:
 
 
 class Fp8Rows:
-    """Rows [T, K] as e4m3 values ``q`` and float32 ``scales`` [T, ceil(K / 128)]: what the products take."""
-    __slots__ = ("q", "scales")
+    """Rows [T, K] as e4m3 values ``q`` and float32 ``scales`` [T, ceil(K / 128)]: what the products take.  Rows that a kernel makes
+    lie in one buffer, the values first; ``q`` and ``scales`` are views of it."""
+    __slots__ = ("shape", "pointers", "index", "_q", "_scales", "_buffer")
 
     def __init__(self, q: torch.Tensor, scales: torch.Tensor):
         if q.dtype != E4M3 or q.dim() != 2 or scales.dtype != torch.float32 or tuple(scales.shape) != (q.shape[0], _blocks(q.shape[1])):
@@ -127,27 +132,45 @@ class Fp8Rows:
                     f"{scales.dtype} {tuple(scales.shape)}")
         if q.shape[1] == 0 or q.shape[1] % 16:
             _refuse(f"8-bit rows have a multiple of 16 columns, got {q.shape[1]}")
-        self.q, self.scales = q, scales
+        if q.device != scales.device or not q.is_contiguous() or not scales.is_contiguous() or q.data_ptr() % 16:
+            _refuse("8-bit rows and their scales are contiguous on one device, the rows 16-byte aligned")
+        self.shape, self._q, self._scales, self._buffer = q.shape, q, scales, None
+        self.pointers, self.index = (q.data_ptr(), scales.data_ptr()), q.get_device()
 
     @property
-    def shape(self):
-        return self.q.shape
+    def q(self) -> torch.Tensor:
+        if self._q is None:
+            rows, k = self.shape
+            self._q = self._buffer[:rows * k].view(E4M3).view(rows, k)
+        return self._q
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            rows, k = self.shape
+            self._scales = self._buffer[rows * k:rows * k + 4 * rows * _blocks(k)].view(torch.float32).view(rows, _blocks(k))
+        return self._scales
 
     @property
     def dtype(self):
-        return self.q.dtype
+        return E4M3
 
     @property
     def device(self):
-        return self.q.device
+        return (self._q if self._buffer is None else self._buffer).device
 
     def values(self) -> torch.Tensor:
-        columns = torch.arange(self.q.shape[1], device=self.q.device) // BLOCK
+        """The float32 numbers that the rows stand for (for tests and comparisons)."""
+        columns = torch.arange(self.shape[1], device=self.device) // BLOCK
         return self.q.to(torch.float32) * self.scales[:, columns]
 
 
 def _empty_rows(rows: int, k: int, device) -> Fp8Rows:
-    return Fp8Rows(torch.empty((rows, k), dtype=E4M3, device=device), torch.empty((rows, _blocks(k)), dtype=torch.float32, device=device))
+    made = Fp8Rows.__new__(Fp8Rows)              # right by construction
+    made._buffer = buffer = torch.empty(rows * k + 4 * rows * -(-k // BLOCK), dtype=torch.uint8, device=device)
+    at = buffer.data_ptr()
+    made.shape, made.pointers, made.index, made._q, made._scales = (rows, k), (at, at + rows * k), buffer.get_device(), None, None
+    return made
 
 
 def _columns(k: int) -> None:
@@ -179,7 +202,7 @@ def quantize_rows_fp8(x: torch.Tensor) -> Fp8Rows:
         _refuse(f"rows are a matrix, got {tuple(x.shape)}")
     _columns(x.shape[1])
     out = _empty_rows(x.shape[0], x.shape[1], x.device)
-    ops._check(ops.lib().tllm_fp8_rows(ops._p(x), ops._dt(x), ops._p(out.q), ops._p(out.scales), x.shape[0], x.shape[1], ops._stream()), "fp8_rows")
+    ops._check(ops.lib().tllm_fp8_rows(ops._p(x), ops._dt(x), *out.pointers, x.shape[0], x.shape[1], ops._stream()), "fp8_rows")
     return out
 
 
@@ -193,127 +216,121 @@ def add_rmsnorm_fp8(h: torch.Tensor, delta: Optional[torch.Tensor], gain: torch.
     _columns(h.shape[1])
     out = _empty_rows(h.shape[0], h.shape[1], h.device)
     ops._check(ops.lib().tllm_add_rmsnorm_fp8(ops._p(h), ops._p(delta), ops.BF16 if delta is None else ops._dt(delta), ops._p(gain), ops._dt(gain),
-                                              float(eps), ops._p(out.q), ops._p(out.scales), h.shape[0], h.shape[1], ops._stream()),
+                                              float(eps), *out.pointers, h.shape[0], h.shape[1], ops._stream()),
                "add_rmsnorm_fp8")
     return out
 
 
 SKINNY_ROWS = 16         # up to this many rows the weight-streaming kernel
 SKINNY_INSIDE_K = 4096   # up to this many columns it rounds eight bfloat16 rows itself
+SKINNY, TILES, PAIRS = 0, 1, 2           # routes of csrc/fp8_product.cu
+ROWS8, INSIDE = 2, 3                     # kinds of rows there, beside float32 and bfloat16
 
 
 def _plan(rows: int, n: int, k: int, sms: int):
-    """(whether pairs of SMs take tiles of 256 x 256, shares of K, blocks per share) of the tensor-core kernels."""
+    """(route, shares of K, blocks per share) of a product with ``n`` weight rows on the tensor cores."""
     kb = _blocks(k)
     if -(-rows // 256) * -(-n // 256) >= sms // 4:
-        return True, 1, kb
+        return PAIRS, 1, kb
     tiles = _blocks(rows) * _blocks(n)
     splits = max(1, min(sms // tiles, kb // 2))
     each = -(-kb // splits)
-    return False, -(-kb // each), each
+    return TILES, -(-kb // each), each
 
 
-def _sums(x: Fp8Rows, weight: Fp8Weight, plan):
-    """The product's float32 shares [splits, T, N]."""
-    ops = _ops()
-    rows, k = x.shape
-    n = weight.shape[0]
-    _, splits, each = plan
-    shares = torch.empty((splits, rows, n), dtype=torch.float32, device=x.device)
-    ops.tcgen05_calls += 1
-    ops._check(ops.lib().tllm_fp8_tcgen05(ops._p(x.q), ops._p(x.scales), ops._p(weight.q), ops._p(weight.scales), ops._p(shares), None, rows, n, k, 1,
-                                          int(weight.gated), 0, splits, each, 0, 0.0, 0.0, ops._p(ops.error_word(x.device)),
-                                          ops._stream()), "fp8_tcgen05")
-    return shares
-
-
-def _check_product(x, weight: Fp8Weight) -> None:
-    if isinstance(x, Fp8Rows):
-        _here(x.q, x.scales, weight.q, weight.scales)
-        if x.q.data_ptr() % 16:
-            _refuse("8-bit rows must be 16-byte aligned")
+@functools.lru_cache(maxsize=8192)
+def _call(rows: int, n: int, k: int, kind: int, gated: bool, to_float: bool, sms: int):
+    """(kind of rows, route, shares, blocks per share, bytes of scratch, kernels) of a product."""
+    if rows <= SKINNY_ROWS:
+        route, splits, each = SKINNY, 1, _blocks(k)
+        if kind == 1 and rows <= 8 and k <= SKINNY_INSIDE_K:
+            kind = INSIDE
     else:
-        _here(x, weight.q, weight.scales)
-        if x.dtype not in (torch.bfloat16, torch.float32) or x.dim() != 2:
+        route, splits, each = _plan(rows, n, k, sms)
+        if route == PAIRS and to_float:          # pairs write bfloat16 or, gated, 8 bits
+            route = TILES
+    scratch = 0 if kind in (ROWS8, INSIDE) else rows * k + -(-4 * rows * _blocks(k) // 16) * 16
+    kernels = 1 + (kind not in (ROWS8, INSIDE))
+    if gated:
+        if route != PAIRS:
+            scratch += 4 * rows * (n // 2 if route == SKINNY else splits * n)
+            kernels += 1
+    elif route == TILES and (splits > 1 or to_float):
+        scratch += 4 * splits * rows * n
+        kernels += 1
+    return kind, route, splits, each, scratch, kernels
+
+
+def _rows_and_weight(x, weight: Fp8Weight):
+    """(rows, columns, kind, values, scales) of rows that may meet the weight."""
+    ops = _ops()
+    if type(x) is Fp8Rows:
+        kind, (values, scales), index = ROWS8, x.pointers, x.index
+    else:
+        if not x.is_cuda or not x.is_contiguous():
+            _refuse("kernels take contiguous CUDA tensors")
+        kind = ops._DT.get(x.dtype)
+        if kind is None or x.dim() != 2:
             _refuse(f"a product with an 8-bit weight takes rows in bfloat16, float32 or 8 bits, got {x.dtype} {tuple(x.shape)}")
-        if x.data_ptr() % 16:
+        values, scales, index = x.data_ptr(), None, x.get_device()
+        if values % 16:
             _refuse("rows must be 16-byte aligned")
-    if x.shape[1] != weight.shape[1]:
-        _refuse(f"rows of {x.shape[1]} columns, a weight of {weight.shape[1]}")
+    current = ops._raw_device()
+    if index != current or weight.index != current:
+        _refuse(f"rows of cuda:{index}, a weight of {weight.device}, the current device is cuda:{current}")
+    rows, k = x.shape
+    if k != weight.shape[1]:
+        _refuse(f"rows of {k} columns, a weight of {weight.shape[1]}")
+    return rows, k, kind, values, scales
 
 
 def linear_fp8(x, weight: Fp8Weight, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """y[T, N] = x . weight^T: ``x`` bfloat16, float32 (both rounded to 8 bits per 128 columns) or ``Fp8Rows``; bfloat16 or float32 out
     (default: x's type, bfloat16 for 8-bit rows)."""
     ops = _ops()
-    _check_product(x, weight)
+    rows, k, kind, values, scales = _rows_and_weight(x, weight)
     if weight.gated:
         _refuse("a gated weight belongs to linear_swiglu")
-    want = out_dtype or (x.dtype if x.dtype in ops._DT else torch.bfloat16)
-    if want not in ops._DT:
+    want = out_dtype or (torch.bfloat16 if kind == ROWS8 else x.dtype)
+    code = ops._DT.get(want)
+    if code is None:
         _refuse(f"unsupported dtype {want}")
-    rows, k = x.shape
-    n = weight.shape[0]
-    y = torch.empty((rows, n), dtype=want, device=x.device)
+    n, device = weight.shape[0], weight.q.device
+    y = torch.empty((rows, n), dtype=want, device=device)
     if rows == 0:
         return y
-    if rows <= SKINNY_ROWS:
-        inside = not isinstance(x, Fp8Rows) and x.dtype == torch.bfloat16 and rows <= 8 and k <= SKINNY_INSIDE_K
-        if not inside and not isinstance(x, Fp8Rows):
-            x = quantize_rows_fp8(x)
-        a, s = (x, None) if inside else (x.q, x.scales)
-        ops._check(ops.lib().tllm_fp8_skinny(ops._p(a), ops._p(s), ops._p(weight.q), ops._p(weight.scales), ops._p(y), ops._DT[want], rows, n, k, 0, 0,
-                                             0.0, 0.0, ops._stream()), "fp8_skinny")
-        return y
-    if not isinstance(x, Fp8Rows):
-        x = quantize_rows_fp8(x)
-    plan = _plan(rows, n, k, ops.SM_COUNT)
-    if plan[1] == 1 and want == torch.bfloat16:
+    kind, route, splits, each, size, kernels = _call(rows, n, k, kind, False, code == 0, ops.SM_COUNT)
+    scratch = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    word = None
+    if route != SKINNY:
+        word = ops.error_word(device).data_ptr()
         ops.tcgen05_calls += 1
-        ops._check(ops.lib().tllm_fp8_tcgen05(ops._p(x.q), ops._p(x.scales), ops._p(weight.q), ops._p(weight.scales), ops._p(y), None, rows, n, k, 0, 0,
-                                              int(plan[0]), 1, plan[2], 0, 0.0, 0.0, ops._p(ops.error_word(x.device)), ops._stream()), "fp8_tcgen05")
-        return y
-    shares = _sums(x, weight, plan)
-    ops._check(ops.lib().tllm_fp8_join(ops._p(shares), plan[1], y.numel(), ops._p(y), ops._DT[want], ops._stream()), "fp8_join")
+    ops._check(ops.lib().tllm_fp8_linear(values, scales, kind, *weight.pointers, y.data_ptr(), code, rows, n, k, route, splits, each,
+                                         scratch.data_ptr() if size else None, word, ops._stream()), "fp8_linear", kernels)
     return y
 
 
 def linear_swiglu_fp8(x, weight: Fp8Weight, act: str = "silu", consts=None) -> Fp8Rows:
     """act(x . Wg^T) * (x . Wu^T) for a gated 8-bit weight, as 8-bit rows for the product that follows, rounded from float32."""
     ops = _ops()
-    _check_product(x, weight)
+    rows, k, kind, values, scales = _rows_and_weight(x, weight)
     if not weight.gated:
         _refuse("linear_swiglu takes a gated 8-bit weight (gate and up rows interleaved by eight)")
-    rows, k = x.shape
-    n = weight.shape[0]
+    n, device = weight.shape[0], weight.q.device
     inter = n // 2
     _columns(inter)
     limit, slope = ops._consts(act, consts)
-    code = ops.ACTIVATIONS[act]
+    out = _empty_rows(rows, inter, device)
     if rows == 0:
-        return _empty_rows(rows, inter, x.device)
-    if rows <= SKINNY_ROWS:
-        inside = not isinstance(x, Fp8Rows) and x.dtype == torch.bfloat16 and rows <= 8 and k <= SKINNY_INSIDE_K
-        if not inside and not isinstance(x, Fp8Rows):
-            x = quantize_rows_fp8(x)
-        a, s = (x, None) if inside else (x.q, x.scales)
-        y = torch.empty((rows, inter), dtype=torch.float32, device=weight.device)
-        ops._check(ops.lib().tllm_fp8_skinny(ops._p(a), ops._p(s), ops._p(weight.q), ops._p(weight.scales), ops._p(y), ops.F32, rows, inter, k, 1, code,
-                                             limit, slope, ops._stream()), "fp8_skinny")
-        return quantize_rows_fp8(y)
-    if not isinstance(x, Fp8Rows):
-        x = quantize_rows_fp8(x)
-    out = _empty_rows(rows, inter, x.device)
-    plan = _plan(rows, n, k, ops.SM_COUNT)
-    if plan[0]:
-        ops.tcgen05_calls += 1
-        ops._check(ops.lib().tllm_fp8_tcgen05(ops._p(x.q), ops._p(x.scales), ops._p(weight.q), ops._p(weight.scales), ops._p(out.q), ops._p(out.scales),
-                                              rows, n, k, 2, 1, 1, 1, plan[2], code, limit, slope, ops._p(ops.error_word(x.device)),
-                                              ops._stream()), "fp8_tcgen05")
         return out
-    shares = _sums(x, weight, plan)
-    ops._check(ops.lib().tllm_fp8_gated_rows(ops._p(shares), plan[1], ops._p(out.q), ops._p(out.scales), rows, inter, code, limit, slope, ops._stream()),
-               "fp8_gated_rows")
+    kind, route, splits, each, size, kernels = _call(rows, n, k, kind, True, False, ops.SM_COUNT)
+    scratch = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    word = None
+    if route != SKINNY:
+        word = ops.error_word(device).data_ptr()
+        ops.tcgen05_calls += 1
+    ops._check(ops.lib().tllm_fp8_gated(values, scales, kind, *weight.pointers, *out.pointers, rows, inter, k, route, splits, each, ops.ACTIVATIONS[act],
+                                        limit, slope, scratch.data_ptr() if size else None, word, ops._stream()), "fp8_gated", kernels)
     return out
 
 
@@ -335,15 +352,16 @@ def _planes(planes, page_size: int, kv_heads: int, head_dim: int):
     """(keys, values, scales, bytes from page to page) of an 8-bit cache's planes, checked."""
     if len(planes) != 3:
         _refuse(f"an 8-bit cache has planes of keys, values and scales, got {len(planes)}")
-    for plane, width in zip(planes, (head_dim, head_dim, SCALE_BYTES)):
-        if not plane.is_cuda or plane.dtype != torch.uint8 or tuple(plane.shape[1:]) != (kv_heads, page_size, width):
-            _refuse(f"an 8-bit cache's plane is uint8 [pages, {kv_heads}, {page_size}, {width}], got {plane.dtype} {tuple(plane.shape)}")
-        if plane.stride()[1:] != (page_size * width, width, 1) or plane.stride(0) != planes[0].stride(0) or plane.shape[0] != planes[0].shape[0]:
-            _refuse("an 8-bit cache's planes are dense within a page and equally far apart")
-        if plane.device.index != torch.cuda.current_device():
-            _refuse(f"a tensor of {plane.device}, the current device is cuda:{torch.cuda.current_device()}")
     k, v, s = planes
-    return k.data_ptr(), v.data_ptr(), s.data_ptr(), k.stride(0)
+    apart, pages, current = k.stride(0), k.shape[0], _ops()._raw_device()
+    for plane, width in ((k, head_dim), (v, head_dim), (s, SCALE_BYTES)):
+        if not plane.is_cuda or plane.dtype is not torch.uint8 or plane.shape != (pages, kv_heads, page_size, width):
+            _refuse(f"an 8-bit cache's plane is uint8 [pages, {kv_heads}, {page_size}, {width}], got {plane.dtype} {tuple(plane.shape)}")
+        if plane.stride() != (apart, page_size * width, width, 1):
+            _refuse("an 8-bit cache's planes are dense within a page and equally far apart")
+        if plane.get_device() != current:
+            _refuse(f"a tensor of {plane.device}, the current device is cuda:{current}")
+    return k.data_ptr(), v.data_ptr(), s.data_ptr(), apart
 
 
 def _int32(what: str, *tensors) -> None:
