@@ -110,35 +110,22 @@ __device__ __forceinline__ void join_runs(const float* m, int me, const float* o
     }
 }
 
-// NT: eights of query heads per key/value head.
+// One run: units [unit0, unit_end) of the keys of one (row, key/value head), by the four warps of a block in turn.  Leaves the warps' results
+// in shared memory (os, ms; every thread may read them): run_sums adds them.  NT: eights of query heads per key/value head.
+// lo, base: the first key that counts, and the same rounded down to 16 (16 keys never straddle a page), where unit 0 begins.
+struct A8Row {
+    const bf16* q;                // of the group's first head
+    const int* table;
+    int g, group, page_size, kv_heads, pos, lo, base;
+    float scale_log2e;
+};
 template <int HD, int NT>
-__global__ void __launch_bounds__(kA8Warps * 32, NT == 1 ? 3 : 2)
-attention_fp8_decode_kernel(const bf16* q, const A8Cache cache, const int* __restrict__ positions, const int* __restrict__ token_slot,
-                            const int* __restrict__ rows, const int* __restrict__ block_table, int max_pages, int page_size, int q_heads,
-                            int kv_heads, int window, float scale_log2e, int splits, float* __restrict__ part_o,
-                            float* __restrict__ part_m, bf16* __restrict__ out) {
-    extern __shared__ __align__(128) unsigned char smem[];
-    TLLM_PDL_ENTER();
+__device__ __forceinline__ void attend_run(unsigned char* smem, const A8Row& row_of, const A8Cache& cache, int unit0, int unit_end) {
     using Unit = A8Unit<HD>;
-    const int split = blockIdx.x, g = blockIdx.y, ridx = blockIdx.z;
-    const int r = rows ? rows[ridx] : ridx;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3, gr = lane >> 2;
-    const int group = q_heads / kv_heads;
-    const int slot = token_slot[r];
-    if (slot < 0) {
-        if (splits == 1)
-            for (int i = threadIdx.x; i < group * HD; i += blockDim.x) out[((size_t)r * q_heads + (size_t)g * group) * HD + i] = __float2bfloat16_rn(0.0f);
-        return;
-    }
-    const int pos = positions[r];
-    const int lo = (window > 0 && pos - window + 1 > 0) ? pos - window + 1 : 0;
-    const int base = lo / 16 * 16;                                 // 16 keys never straddle a page
-    const int units_all = (pos - base) / kA8Unit + 1;
-    int per = (units_all + splits - 1) / splits;
-    per = (per + kA8Warps - 1) / kA8Warps * kA8Warps;              // whole rounds of the four warps
-    const int unit_end = min(units_all, split * per + per);
-    int unit = split * per + warp;
-    const int* table = block_table + (size_t)slot * max_pages;
+    const int g = row_of.g, group = row_of.group, page_size = row_of.page_size, pos = row_of.pos, lo = row_of.lo, base = row_of.base;
+    const int* table = row_of.table;
+    int unit = unit0 + warp;
     unsigned char* ring = smem + (size_t)warp * kA8Stages * Unit::kBytes;
 
     // ---- the next unit to fetch: its first key, that key's page (index in the table) and place in it, for both of its sixteens
@@ -149,6 +136,14 @@ attention_fp8_decode_kernel(const bf16* q, const A8Cache cache, const int* __res
     const uint8_t* const k0 = cache.k + lane * 16;
     const uint8_t* const v0 = cache.v + lane * 16;
     const int key_dst = Unit::key_at(lane / (HD / 16), lane % (HD / 16));
+    // its two pages are looked up a unit ahead, so that no copy waits for the table
+    int page[2];
+    auto look_up = [&]() {
+        const bool there = f_unit < unit_end, wraps = in_page + 16 >= page_size;
+        page[0] = there ? table[page_at] : -1;                                     // its first key is at or before pos
+        page[1] = there && key0 + 16 <= pos ? (wraps ? table[page_at + 1] : page[0]) : -1;
+    };
+    look_up();
     auto fetch = [&]() {
         if (f_unit < unit_end) {
             const bool wraps = in_page + 16 >= page_size;
@@ -156,19 +151,18 @@ attention_fp8_decode_kernel(const bf16* q, const A8Cache cache, const int* __res
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int first = key0 + 16 * h;
-                const int page = first <= pos ? table[h && wraps ? page_at + 1 : page_at] : -1;
-                const size_t at = (size_t)max(page, 0) * cache.stride, token = (size_t)g * page_size + (h == 0 ? in_page : wraps ? in_page + 16 - page_size : in_page + 16);
+                const size_t at = (size_t)max(page[h], 0) * cache.stride, token = (size_t)g * page_size + (h == 0 ? in_page : wraps ? in_page + 16 - page_size : in_page + 16);
                 const uint8_t *kp = k0 + at + token * HD, *vp = v0 + at + token * HD;
-                const bool whole = page >= 0 && first >= lo && first + 15 <= pos;
+                const bool whole = page[h] >= 0 && first >= lo && first + 15 <= pos;
                 constexpr int kPieces = 16 * HD / 16 / 32;         // per lane: 4 or 2
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) {
                     const int n = lane + 32 * i, row = n / (HD / 16), chunk = n % (HD / 16);
-                    const bool ok = whole || (page >= 0 && first + row >= lo && first + row <= pos);
+                    const bool ok = whole || (page[h] >= 0 && first + row >= lo && first + row <= pos);
                     cp_async_16(dst + key_dst + h * 16 * HD + i * 512, kp + i * 512, ok);
                     cp_async_16(dst + Unit::kPlane + Unit::value_at(row, chunk) + h * 16 * HD, vp + i * 512, ok);
                 }
-                if (lane < 8) cp_async_16(dst + 2 * Unit::kPlane + h * 128 + lane * 16, cache.scales + at + token * 8 + lane * 16, page >= 0);   // masked below
+                if (lane < 8) cp_async_16(dst + 2 * Unit::kPlane + h * 128 + lane * 16, cache.scales + at + token * 8 + lane * 16, page[h] >= 0);   // masked below
             }
             f_unit += kA8Warps;
             key0 += kStep;
@@ -176,6 +170,7 @@ attention_fp8_decode_kernel(const bf16* q, const A8Cache cache, const int* __res
             in_page += step_rest;
             if (in_page >= page_size) in_page -= page_size, ++page_at;
             f_stage = f_stage + 1 == kA8Stages ? 0 : f_stage + 1;
+            look_up();
         }
         cp_async_commit();                                         // one group per call, empty past the end
     };
@@ -188,7 +183,7 @@ attention_fp8_decode_kernel(const bf16* q, const A8Cache cache, const int* __res
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int head = nt * 8 + gr;
-        const bf16* qp = q + ((size_t)r * q_heads + (size_t)g * group + min(head, group - 1)) * HD;
+        const bf16* qp = row_of.q + (size_t)min(head, group - 1) * HD;
         float v[HD / 4];
         float largest = 0.0f;
 #pragma unroll
@@ -211,7 +206,7 @@ attention_fp8_decode_kernel(const bf16* q, const A8Cache cache, const int* __res
         const int shift = e == 255 ? 0 : 14 + 127 - max(e, 1);     // -113 .. 140
         const float f0 = __int_as_float((127 + shift / 2) << 23), f1 = __int_as_float((127 + shift - shift / 2) << 23);
         const float b0 = __int_as_float((127 - shift / 2) << 23), b1 = __int_as_float((127 - (shift - shift / 2)) << 23);
-        const float back = scale_log2e * b0 * b1;
+        const float back = row_of.scale_log2e * b0 * b1;
         const bool live = head < group;
 #pragma unroll
         for (int f = 0; f < HD / 16; ++f) {
@@ -378,99 +373,291 @@ attention_fp8_decode_kernel(const bf16* q, const A8Cache cache, const int* __res
             }
         }
     __syncthreads();
-    for (int idx = threadIdx.x; idx < group * HD; idx += blockDim.x) {
-        const int row = idx / HD, d = idx - row * HD;
+}
+
+// Head `row` of the group and dim d of a run: the warps' results added (join_runs).
+template <int HD, int NT>
+__device__ __forceinline__ void run_sums(const unsigned char* smem, int row, int d, float& acc, float& total, float& mm, float& dn) {
+    const float* os = reinterpret_cast<const float*>(smem);
+    const float* ms = os + kA8Warps * 8 * NT * HD;
+    join_runs<kA8Warps>(ms + row * 3, 8 * NT * 3, os + (size_t)row * HD + d, 8 * NT * HD, kA8Warps, acc, total, mm, dn);
+}
+
+// Units of 32 keys that a row's position and window give it.
+__device__ __forceinline__ int first_key(int pos, int window) { return window > 0 && pos - window + 1 > 0 ? pos - window + 1 : 0; }
+__device__ __forceinline__ int units_of(int pos, int window) { return (pos - first_key(pos, window) / 16 * 16) / kA8Unit + 1; }
+
+struct A8Step {
+    const bf16* q;
+    A8Cache cache;
+    const int *positions, *token_slot, *rows, *block_table;
+    int n_rows, max_pages, page_size, q_heads, kv_heads, window;
+    float scale_log2e;
+};
+template <int HD>
+__device__ __forceinline__ A8Row row_at(const A8Step& st, int r, int slot, int g) {
+    A8Row x;
+    x.group = st.q_heads / st.kv_heads;
+    x.g = g;
+    x.q = st.q + ((size_t)r * st.q_heads + (size_t)g * x.group) * HD;
+    x.table = st.block_table + (size_t)slot * st.max_pages;
+    x.page_size = st.page_size;
+    x.kv_heads = st.kv_heads;
+    x.pos = st.positions[r];
+    x.lo = first_key(x.pos, st.window);
+    x.base = x.lo / 16 * 16;
+    x.scale_log2e = st.scale_log2e;
+    return x;
+}
+
+// Short contexts: a block of threads per (row, key/value head), the whole of it one run.
+template <int HD, int NT>
+__global__ void __launch_bounds__(kA8Warps * 32, NT == 1 ? 3 : 2) attention_fp8_whole_kernel(const A8Step st, bf16* __restrict__ out) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    TLLM_PDL_ENTER();
+    const int g = blockIdx.x, ridx = blockIdx.y;
+    const int r = st.rows ? st.rows[ridx] : ridx, group = st.q_heads / st.kv_heads;
+    const int slot = st.token_slot[r];
+    bf16* dst = out + ((size_t)r * st.q_heads + (size_t)g * group) * HD;
+    if (slot < 0) {
+        for (int i = threadIdx.x; i < group * HD; i += blockDim.x) dst[i] = __float2bfloat16_rn(0.0f);
+        return;
+    }
+    const A8Row x = row_at<HD>(st, r, slot, g);
+    attend_run<HD, NT>(smem, x, st.cache, 0, units_of(x.pos, st.window));
+    for (int i = threadIdx.x; i < group * HD; i += blockDim.x) {
         float acc, total, mm, dn;
-        join_runs<kA8Warps>(ms + row * 3, 8 * NT * 3, os + (size_t)row * HD + d, 8 * NT * HD, kA8Warps, acc, total, mm, dn);
-        const int head = g * group + row;
-        if (splits == 1) {
-            const float up = dn == -INFINITY ? 0.0f : exp2f(dn - kA8Lift);
-            out[((size_t)r * q_heads + head) * HD + d] = __float2bfloat16_rn(acc * up / total);
-        } else {
-            const size_t at = ((size_t)ridx * q_heads + head) * splits + split;
-            part_o[at * HD + d] = acc;
-            if (d == 0) { part_m[at * 3] = mm; part_m[at * 3 + 1] = dn; part_m[at * 3 + 2] = total; }
-        }
+        run_sums<HD, NT>(smem, i / HD, i % HD, acc, total, mm, dn);
+        dst[i] = __float2bfloat16_rn(acc * (dn == -INFINITY ? 0.0f : exp2f(dn - kA8Lift)) / total);
     }
 }
 
-// The runs of a (row, head) added.  Every warp finds the runs' factors, a lane each for every 32nd run; then the block's kA8JoinGroups groups of HD
-// threads add every kA8JoinGroups-th run's values, eight of them on their way at once, and the groups' sums are added in order.  (One thread per dim
-// that walked over 64 runs one by one took 43 us.)
-constexpr int kA8JoinGroups = 4, kA8MaxRuns = 128;
-template <int HD>
-__global__ void __launch_bounds__(HD * kA8JoinGroups)
-attention_fp8_join_kernel(const float* part_o, const float* part_m, const int* __restrict__ token_slot, const int* __restrict__ rows, int q_heads,
-                          int splits, bf16* __restrict__ out) {
-    __shared__ float factor[kA8MaxRuns], sums[kA8JoinGroups][HD];
+// Longer ones: the keys of all rows shared by all blocks of threads, whatever the rows' lengths, in one of two ways.
+//   Chunks, where there are two blocks and more for every (row, head): each is cut into chunks of `each` units, the shortest that leave no chunk
+//   without a block, and a block takes one.
+//   Shares, where there are more (rows, heads) than that: all units in a row, (row, head, unit), are cut into equal shares; a share is the end of
+//   one (row, head), whole ones, and the beginning of another.
+// A (row, head) that one block has whole is written; pieces go to scratch.  Place of a chunk: its block; of the piece of (row, head) i in share b:
+// i + b (no two pieces have the same, as every next piece is of the next pair, the next share or both).  Chunks and shares are whole rounds of the
+// four warps.  plan: the chunks (units) of a head before each row, then 0 (the length of a share): the first block leaves it for the kernel
+// that adds the pieces.  (A grid of equal runs per row, whose lengths differ: 64 rows of 1000 to 4096 keys 86 us however finely cut, in shares 78;
+// shares alone, 8 rows of 500 to 2000 keys 21 us, as some blocks work on two pieces one after the other, in chunks 15.)
+constexpr int kA8MaxRows = 512, kA8MaxShares = 512;
+template <int HD, int NT>
+__global__ void __launch_bounds__(kA8Warps * 32, NT == 1 ? 3 : 2)
+attention_fp8_share_kernel(const A8Step st, int* __restrict__ plan, float* __restrict__ part_o, float* __restrict__ part_m, bf16* __restrict__ out) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ int before[kA8MaxRows + 1], sums[2][kA8Warps];
     TLLM_PDL_ENTER();
-    const int ridx = blockIdx.x, head = blockIdx.y, d = threadIdx.x % HD, group = threadIdx.x / HD, lane = threadIdx.x & 31;
-    const int r = rows ? rows[ridx] : ridx;
-    bf16* dst = out + ((size_t)r * q_heads + head) * HD;
-    if (token_slot[r] < 0) {
-        if (group == 0) dst[d] = __float2bfloat16_rn(0.0f);
-        return;
-    }
-    const size_t base = ((size_t)ridx * q_heads + head) * splits;
-    constexpr int kEach = kA8MaxRuns / 32;
-    float m[kEach], dd[kEach], l[kEach], mm = -INFINITY, dn = -INFINITY, total = 0.0f;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = st.q_heads / st.kv_heads, blocks = gridDim.x;
+    // units of four rows a thread; sums over the block
+    constexpr int kEach = kA8MaxRows / (kA8Warps * 32);
+    int units[kEach], some = 0, rows_here = 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-        const int s = lane + 32 * i;
-        const float* e = part_m + (base + s) * 3;
-        const bool there = s < splits;
-        m[i] = there ? e[0] : -INFINITY;
-        dd[i] = there ? e[1] : -INFINITY;
-        l[i] = there ? e[2] : 0.0f;
-        mm = fmaxf(mm, m[i]);
+        const int ridx = threadIdx.x * kEach + i;
+        units[i] = 0;
+        if (ridx < st.n_rows) {
+            const int r = st.rows ? st.rows[ridx] : ridx;
+            const int pos = st.positions[r];
+            if (st.token_slot[r] >= 0) units[i] = units_of(pos, st.window);
+        }
+        some += units[i];
+        rows_here += units[i] > 0;
     }
-    mm = warp_max(mm);
-    // a run without keys has M of -infinity and sums of zero; scores that are all NaN leave M so too, and l NaN
+    int turn = 0;
+    auto block_total = [&](int v) {
+        v = __reduce_add_sync(0xffffffffu, v);
+        if (lane == 0) sums[turn][warp] = v;
+        __syncthreads();
+        int t = 0;
+#pragma unroll
+        for (int i = 0; i < kA8Warps; ++i) t += sums[turn][i];
+        turn ^= 1;
+        return t;
+    };
+    const int total = block_total(some) * st.kv_heads;            // below 2^31 - 2^13: see the entry point
+    int each = ((total + blocks - 1) / blocks + kA8Warps - 1) / kA8Warps * kA8Warps;
+    if (each == 0) each = kA8Warps;
+    const bool chunks = block_total(rows_here) * st.kv_heads * 2 <= blocks;
+    if (chunks) {
+        // the shortest of a few lengths, a sixteenth longer each time: with twice as many blocks as pairs, twice the mean length always does
+        for (;;) {
+            int c = 0;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) c += (units[i] + each - 1) / each;
+            if (block_total(c) * st.kv_heads <= blocks) break;
+            each += max(each / 16 / kA8Warps, 1) * kA8Warps;
+        }
+    }
+    // chunks or units of a head before each row
+    int mine[kEach], run = 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-        dd[i] = m[i] == -INFINITY ? -INFINITY : dd[i] + (m[i] - mm);
-        total += m[i] == -INFINITY ? l[i] : l[i] * exp2f(m[i] - mm);
-        dn = fmaxf(dn, dd[i]);
+        mine[i] = run;
+        run += chunks ? (units[i] + each - 1) / each : units[i];
     }
-    dn = warp_max(dn);
-    total = warp_sum(total);
-    if (threadIdx.x < 32)
+    int upto = run;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i)
-            if (lane + 32 * i < splits) factor[lane + 32 * i] = dd[i] == -INFINITY ? 0.0f : exp2f(dd[i] - dn);
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) sums[turn][warp] = upto;
     __syncthreads();
-    float acc = 0.0f;
-    const float* o = part_o + base * HD + d;
-#pragma unroll 8
-    for (int s = group; s < splits; s += kA8JoinGroups) acc = fmaf(o[(size_t)s * HD], factor[s], acc);
-    sums[group][d] = acc;
-    __syncthreads();
-    if (group != 0) return;
+    int offset = upto - run, all = 0;
 #pragma unroll
-    for (int g = 1; g < kA8JoinGroups; ++g) acc += sums[g][d];
-    const float up = dn == -INFINITY ? 0.0f : exp2f(dn - kA8Lift);
-    dst[d] = __float2bfloat16_rn(acc * up / total);
+    for (int i = 0; i < kA8Warps; ++i) {
+        if (i < warp) offset += sums[turn][i];
+        all += sums[turn][i];
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+        if (threadIdx.x * kEach + i < st.n_rows) before[threadIdx.x * kEach + i] = offset + mine[i];
+    if (threadIdx.x == 0) before[st.n_rows] = all;
+    __syncthreads();
+    if (blockIdx.x == 0) {
+        for (int i = threadIdx.x; i <= st.n_rows; i += blockDim.x) plan[i] = before[i];
+        if (threadIdx.x == 0) plan[st.n_rows + 1] = chunks ? 0 : each;
+    }
+    // in chunks or units, of all heads: this block's first and the one behind its last
+    const int here = all * st.kv_heads;
+    if ((long long)blockIdx.x * (chunks ? 1 : each) >= here) return;
+    int at = blockIdx.x * (chunks ? 1 : each);
+    const int end = chunks ? at + 1 : min(at + each, here);
+    // the row that holds it: the last one with before * kv_heads <= at (rows with nothing are passed over)
+    int ridx = 0;
+    for (int step = kA8MaxRows / 2; step > 0; step >>= 1)
+        if (ridx + step < st.n_rows && before[ridx + step] * st.kv_heads <= at) ridx += step;
+    while (at < end) {
+        const int n = before[ridx + 1] - before[ridx];
+        if (n == 0) { ++ridx; continue; }
+        const int in_row = at - before[ridx] * st.kv_heads, g = in_row / n, first = in_row - g * n;
+        const int r = st.rows ? st.rows[ridx] : ridx;
+        const A8Row x = row_at<HD>(st, r, st.token_slot[r], g);
+        const int u0 = chunks ? first * each : first;
+        const int u1 = chunks ? min(u0 + each, units_of(x.pos, st.window)) : min(n, u0 + end - at);
+        attend_run<HD, NT>(smem, x, st.cache, u0, u1);
+        const bool whole = chunks ? n == 1 : u0 == 0 && u1 == n;
+        const size_t place = ((chunks ? (size_t)0 : (size_t)ridx * st.kv_heads + g) + blockIdx.x) * group;
+        for (int i = threadIdx.x; i < group * HD; i += blockDim.x) {
+            const int row = i / HD, d = i % HD;
+            float acc, sum, mm, dn;
+            run_sums<HD, NT>(smem, row, d, acc, sum, mm, dn);
+            if (whole) {
+                out[((size_t)r * st.q_heads + (size_t)g * group) * HD + i] = __float2bfloat16_rn(acc * (dn == -INFINITY ? 0.0f : exp2f(dn - kA8Lift)) / sum);
+            } else {
+                part_o[(place + row) * HD + d] = acc;
+                if (d == 0) { part_m[(place + row) * 3] = mm; part_m[(place + row) * 3 + 1] = dn; part_m[(place + row) * 3 + 2] = sum; }
+            }
+        }
+        if (chunks) return;
+        at += u1 - u0;
+        if (g == st.kv_heads - 1 && u1 == n) ++ridx;
+        __syncthreads();                                           // the ring may be filled again
+    }
+}
+
+// The pieces of a (row, head) added in the order of their keys.  A warp's lanes find the pieces' factors, 32 at a time, and add HD / 32 dims
+// each, four pieces on their way at once.  WIDE (few heads of many pieces): the warps of a block share a head's pieces, and their sums are
+// added in order; else each takes a head of the group.  Rows of no request become zeros here.  (512 threads per head, whatever the pieces,
+// took 18 us for 2048 heads of two pieces each.)
+constexpr int kA8JoinWarps = 8;
+template <int HD, bool WIDE>
+__global__ void __launch_bounds__(kA8JoinWarps * 32)
+attention_fp8_join_kernel(const A8Step st, const int* plan, const float* part_o, const float* part_m, bf16* __restrict__ out) {
+    constexpr int kDims = HD / 32;
+    __shared__ float sums[WIDE ? kA8JoinWarps : 1][HD];
+    TLLM_PDL_ENTER();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5, ridx = blockIdx.y;
+    const int r = st.rows ? st.rows[ridx] : ridx, group = st.q_heads / st.kv_heads, slot = st.token_slot[r];
+    const int before = plan[ridx], n = plan[ridx + 1] - before, each = plan[st.n_rows + 1];
+    const int g = WIDE ? blockIdx.x / group : blockIdx.x;
+    const int start = before * st.kv_heads + g * n, b0 = each == 0 ? start : start / each;
+    const int pieces = each == 0 ? n : (start + n - 1) / each - b0 + 1;
+    if (slot >= 0 && pieces == 1) return;                          // written where it was made
+    const int first = WIDE ? blockIdx.x % group : warp, step = WIDE ? group : warps;
+    for (int h = first; h < group; h += step) {
+        bf16* dst = out + ((size_t)r * st.q_heads + g * group + h) * HD + lane * kDims;
+        if (slot < 0) {
+            if (!WIDE || warp == 0)
+#pragma unroll
+                for (int i = 0; i < kDims; ++i) dst[i] = __float2bfloat16_rn(0.0f);
+            continue;
+        }
+        const size_t base = ((each == 0 ? (size_t)0 : (size_t)ridx * st.kv_heads + g) + b0) * group + h;      // the first piece's place
+        const float* me = part_m + base * 3;
+        const float* oe = part_o + base * HD + lane * kDims;
+        float mm = -INFINITY, dn = -INFINITY, total = 0.0f;
+        for (int p = lane; p < pieces; p += 32) mm = fmaxf(mm, me[p * group * 3]);
+        mm = warp_max(mm);
+        // a piece without keys has M of -infinity and sums of zero; scores that are all NaN leave M so too, and l NaN
+        for (int p = lane; p < pieces; p += 32) {
+            const float m = me[p * group * 3], l = me[p * group * 3 + 2];
+            total += m == -INFINITY ? l : l * exp2f(m - mm);
+            if (m != -INFINITY) dn = fmaxf(dn, me[p * group * 3 + 1] + (m - mm));
+        }
+        dn = warp_max(dn);
+        total = warp_sum(total);
+        float acc[kDims];
+#pragma unroll
+        for (int i = 0; i < kDims; ++i) acc[i] = 0.0f;
+        for (int p0 = 0; p0 < pieces; p0 += 32) {
+            const int p = p0 + lane;
+            const float m = p < pieces ? me[p * group * 3] : -INFINITY;
+            const float of = m == -INFINITY ? -INFINITY : me[p * group * 3 + 1] + (m - mm);
+            const float factor = of == -INFINITY ? 0.0f : exp2f(of - dn);
+            const int count = min(32, pieces - p0);
+#pragma unroll 4
+            for (int i = WIDE ? warp : 0; i < count; i += WIDE ? warps : 1) {
+                const float f = __shfl_sync(0xffffffffu, factor, i);
+                const float* o = oe + (size_t)(p0 + i) * group * HD;
+#pragma unroll
+                for (int e = 0; e < kDims; ++e) acc[e] = fmaf(o[e], f, acc[e]);
+            }
+        }
+        if (WIDE) {
+#pragma unroll
+            for (int e = 0; e < kDims; ++e) sums[warp][lane * kDims + e] = acc[e];
+            __syncthreads();
+            if (warp != 0) return;
+#pragma unroll
+            for (int i = 1; i < kA8JoinWarps; ++i)
+#pragma unroll
+                for (int e = 0; e < kDims; ++e) acc[e] += sums[i][lane * kDims + e];
+        }
+        const float up = dn == -INFINITY ? 0.0f : exp2f(dn - kA8Lift);
+#pragma unroll
+        for (int e = 0; e < kDims; ++e) dst[e] = __float2bfloat16_rn(acc[e] * up / total);
+        if (WIDE) return;
+    }
 }
 
 template <int HD, int NT>
-static int launch_attention_fp8(const void* q, const A8Cache& cache, const int* positions, const int* token_slot, const int* rows, int n_rows,
-                                const int* block_table, int max_pages, int page_size, int q_heads, int kv_heads, int window, float scale,
-                                int splits, float* part_o, float* part_m, void* out, cudaStream_t stream) {
+static int launch_attention_fp8(const A8Step& st, int blocks, int* plan, float* part_o, float* part_m, void* out, cudaStream_t stream) {
     constexpr size_t ring = (size_t)kA8Warps * kA8Stages * A8Unit<HD>::kBytes, joined = (size_t)kA8Warps * 8 * NT * (HD + 3) * sizeof(float);
     constexpr size_t smem = ring > joined ? ring : joined;
     static OncePerDevice configured;
     if (configured.first()) {
-        cudaError_t e = cudaFuncSetAttribute(attention_fp8_decode_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        cudaError_t e = cudaFuncSetAttribute(attention_fp8_whole_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_fp8_share_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) { set_error("attention_fp8_decode: %s", cudaGetErrorString(e)); return (int)e; }
         configured.done();
     }
-    launch_pdl(kPdlAlways, attention_fp8_decode_kernel<HD, NT>, dim3(splits, kv_heads, n_rows), dim3(kA8Warps * 32), smem, stream,
-               (const bf16*)q, cache, positions, token_slot, rows, block_table, max_pages, page_size, q_heads, kv_heads, window,
-               scale * 1.4426950408889634f, splits, part_o, part_m, (bf16*)out);
-    const int rc = finish_launch("attention_fp8_decode");
-    if (rc != 0 || splits == 1) return rc;
-    launch_pdl(kPdlAlways, attention_fp8_join_kernel<HD>, dim3(n_rows, q_heads), dim3(HD * kA8JoinGroups), 0, stream, (const float*)part_o, (const float*)part_m,
-               token_slot, rows, q_heads, splits, (bf16*)out);
+    if (blocks == 0) {
+        launch_pdl(kPdlAlways, attention_fp8_whole_kernel<HD, NT>, dim3(st.kv_heads, st.n_rows), dim3(kA8Warps * 32), smem, stream, st, (bf16*)out);
+        return finish_launch("attention_fp8_whole");
+    }
+    launch_pdl(kPdlAlways, attention_fp8_share_kernel<HD, NT>, dim3(blocks), dim3(kA8Warps * 32), smem, stream, st, plan, part_o, part_m, (bf16*)out);
+    const int rc = finish_launch("attention_fp8_share");
+    if (rc != 0) return rc;
+    const int group = st.q_heads / st.kv_heads;
+    if ((long long)st.n_rows * st.kv_heads * 8 <= blocks)         // eight pieces a head and more, on average
+        launch_pdl(kPdlAlways, attention_fp8_join_kernel<HD, true>, dim3(st.q_heads, st.n_rows), dim3(kA8JoinWarps * 32), 0, stream, st,
+                   (const int*)plan, (const float*)part_o, (const float*)part_m, (bf16*)out);
+    else
+        launch_pdl(kPdlAlways, attention_fp8_join_kernel<HD, false>, dim3(st.kv_heads, st.n_rows), dim3((group < kA8JoinWarps ? group : kA8JoinWarps) * 32),
+                   0, stream, st, (const int*)plan, (const float*)part_o, (const float*)part_m, (bf16*)out);
     return finish_launch("attention_fp8_join");
 }
 
@@ -540,30 +727,36 @@ static int check_a8(const char* what, const void* k, const void* v, const void* 
 }
 
 // q, out [rows, q_heads * head_dim] bfloat16; planes of pages `page_bytes` apart: k, v [kv_heads][page_size][head_dim] e4m3, scales
-// [kv_heads][page_size][2] float32.  rows: indices of the one-token rows, null for 0 .. n_rows - 1.  Scratch for splits > 1: part_o
-// float[n_rows * q_heads * splits * head_dim], part_m float[n_rows * q_heads * splits * 3].
+// [kv_heads][page_size][2] float32.  rows: indices of the one-token rows, null for 0 .. n_rows - 1.  blocks: 0 for a block of threads per (row,
+// key/value head), else how many share all rows' keys (at most 512 rows and 512 blocks); then scratch, 16-byte aligned: float [(n_rows * kv_heads + blocks) *
+// (q_heads / kv_heads) * (head_dim + 3)], int [n_rows + 2].
 extern "C" int tllm_attention_fp8_decode(const void* q, const void* k, const void* v, const void* scales, long long page_bytes,
                                          const int* positions, const int* token_slot, const int* rows, int n_rows, const int* block_table,
                                          int max_pages, int page_size, int q_heads, int kv_heads, int head_dim, int window, float scale,
-                                         int splits, float* part_o, float* part_m, void* out, cudaStream_t stream) {
+                                         int blocks, float* scratch, void* out, cudaStream_t stream) {
     if (check_a8("attention_fp8_decode", k, v, scales, page_bytes, page_size, kv_heads, head_dim) != 0) return -1;
     TLLM_REQUIRE(q_heads > 0 && q_heads % kv_heads == 0 && q_heads / kv_heads <= 16,
                  "attention_fp8_decode: %d query heads over %d key/value heads (at most 16 per group)", q_heads, kv_heads);
-    TLLM_REQUIRE(splits >= 1 && splits <= kA8MaxRuns && n_rows >= 0 && n_rows <= 65535 && q_heads <= 65535 && max_pages > 0, "attention_fp8_decode: bad grid");
-    TLLM_REQUIRE(splits == 1 || (part_o && part_m), "attention_fp8_decode: %d runs of keys need scratch", splits);
-    TLLM_REQUIRE(q && out && positions && token_slot && block_table && (reinterpret_cast<uintptr_t>(q) & 15u) == 0,
+    TLLM_REQUIRE(n_rows >= 0 && n_rows <= 65535 && q_heads <= 65535 && max_pages > 0 && window >= 0, "attention_fp8_decode: bad grid");
+    TLLM_REQUIRE(blocks >= 0 && blocks <= kA8MaxShares && (blocks == 0 || (n_rows <= kA8MaxRows && scratch)),
+                 "attention_fp8_decode: %d rows shared by %d blocks (at most 512 and 512, with scratch)", n_rows, blocks);
+    TLLM_REQUIRE(blocks == 0 || (long long)n_rows * kv_heads * ((long long)max_pages * page_size / kA8Unit + 1) < 0x7fffffff - (1 << 13),
+                 "attention_fp8_decode: too many keys for shares");
+    TLLM_REQUIRE(q && out && positions && token_slot && block_table && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(scratch)) & 15u) == 0,
                  "attention_fp8_decode: missing or unaligned operands");
     if (n_rows == 0) return 0;
-    const A8Cache cache{(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)scales, page_bytes};
-#define ATTEND(HD, NT)                                                                                                                       \
-    return launch_attention_fp8<HD, NT>(q, cache, positions, token_slot, rows, n_rows, block_table, max_pages, page_size, q_heads, kv_heads, \
-                                        window, scale, splits, part_o, part_m, out, stream)
-    const bool one = q_heads / kv_heads <= 8;
+    const A8Step st{(const bf16*)q, A8Cache{(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)scales, page_bytes}, positions, token_slot, rows,
+                    block_table, n_rows, max_pages, page_size, q_heads, kv_heads, window, scale * 1.4426950408889634f};
+    const int group = q_heads / kv_heads;
+    const size_t places = ((size_t)n_rows * kv_heads + blocks) * group;
+    float *part_o = scratch, *part_m = scratch + places * head_dim;
+    int* plan = reinterpret_cast<int*>(part_m + places * 3);
+#define ATTEND(HD, NT) return launch_attention_fp8<HD, NT>(st, blocks, plan, part_o, part_m, out, stream)
     if (head_dim == 64) {
-        if (one) ATTEND(64, 1);
+        if (group <= 8) ATTEND(64, 1);
         ATTEND(64, 2);
     }
-    if (one) ATTEND(128, 1);
+    if (group <= 8) ATTEND(128, 1);
     ATTEND(128, 2);
 #undef ATTEND
 }

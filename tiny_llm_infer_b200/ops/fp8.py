@@ -47,7 +47,7 @@ def declare(h) -> None:
         "tllm_fp8_weight": [vp, i32, vp, vp, i32, i32, i32, vp],
         "tllm_qk_norm_rope_store_fp8": [vp, vp, vp, i32, f32, vp, i32, vp, vp, vp, i32, vp, vp, vp, i64, i32, vp, i32, i32, i32, i32, i32,
                                         vp, vp],
-        "tllm_attention_fp8_decode": [vp, vp, vp, vp, i64, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, f32, i32, vp, vp, vp, vp],
+        "tllm_attention_fp8_decode": [vp, vp, vp, vp, i64, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, f32, i32, vp, vp, vp],
         "tllm_attention_fp8_unpack": [vp, vp, vp, i64, vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp],
     }
     for name, args in sigs.items():
@@ -403,35 +403,48 @@ def qk_norm_rope_store_fp8(qkv: torch.Tensor, q_gain, k_gain, eps: float, inv_fr
 
 def _attention_operands(what, q, out, positions, token_slot, rows, n_rows, block_table, q_heads, kv_heads, head_dim) -> None:
     _here(q, out, positions, token_slot, rows, block_table)
-    _int32(what, positions, token_slot, rows, block_table)
-    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or q.dim() != 2 or q.shape[1] != q_heads * head_dim or out.shape != q.shape:
-        _refuse(f"{what}: queries and outputs are bfloat16 [rows, {q_heads * head_dim}], got {q.dtype} {tuple(q.shape)} and {out.dtype} {tuple(out.shape)}")
-    if n_rows > (q.shape[0] if rows is None else rows.numel()) or min(positions.numel(), token_slot.numel()) < q.shape[0]:
-        _refuse(f"{what}: {n_rows} rows of {q.shape[0]}, a position and a slot for each")
+    if not positions.dtype is token_slot.dtype is block_table.dtype is torch.int32 or (rows is not None and rows.dtype is not torch.int32):
+        _refuse(f"{what}: positions, slots, rows and block tables are int32")
+    shape = q.shape
+    if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16 or len(shape) != 2 or shape[1] != q_heads * head_dim or out.shape != shape:
+        _refuse(f"{what}: queries and outputs are bfloat16 [rows, {q_heads * head_dim}], got {q.dtype} {tuple(shape)} and {out.dtype} {tuple(out.shape)}")
+    if n_rows > (shape[0] if rows is None else rows.numel()) or positions.numel() < shape[0] or token_slot.numel() < shape[0]:
+        _refuse(f"{what}: {n_rows} rows of {shape[0]}, a position and a slot for each")
+
+
+SHARED_ROWS = 512        # at most so many rows share blocks
+SHARED_FROM = 512        # and only where a row may see more keys than this
+
+
+def attention_blocks(rows: int, kv_heads: int, group: int, reach: int, sms: int) -> int:
+    """Blocks of threads that share all rows' keys in ``paged_attention_decode_fp8``, or 0 for one block per (row, key/value head) and no
+    second kernel."""
+    if rows > SHARED_ROWS or reach <= SHARED_FROM:
+        return 0
+    return (3 if group <= 8 else 2) * sms                    # what is resident at once
 
 
 def paged_attention_decode_fp8(q, planes, positions, token_slot, rows, n_rows, block_table, page_size, q_heads, kv_heads, head_dim, window, scale,
-                               out, max_context, splits=None):
+                               out, max_context, blocks=None):
     """Attention of one-token rows (``rows``: their indices, None for the first ``n_rows``) over an 8-bit paged cache, ``planes`` =
-    (keys, values, scales): positions max(0, pos - window + 1) .. pos of the row's own request.  Keys are split over ``splits`` blocks per
-    (row, key/value head), whose results a second kernel adds in order.  Rows with a negative slot become zeros; rows of ``out``
-    that are not asked for stay as they are.  ``max_context``: no row's position is at or behind it."""
+    (keys, values, scales): positions max(0, pos - window + 1) .. pos of the row's own request.  All rows' keys are cut into as many equal
+    shares as there are ``blocks`` of threads, and a second kernel adds the pieces of a row in their order (0: one block per (row, key/value head),
+    one kernel; None: by ``attention_blocks``).  Rows with a negative slot become zeros; rows of ``out`` that are not asked for
+    stay as they are.  ``max_context``: no row's position is at or behind it (it sizes the grid)."""
     ops = _ops()
     _attention_operands("paged_attention_decode_fp8", q, out, positions, token_slot, rows, n_rows, block_table, q_heads, kv_heads, head_dim)
     k, v, s, stride = _planes(planes, page_size, kv_heads, head_dim)
-    if max_context > block_table.shape[1] * page_size:
-        max_context = block_table.shape[1] * page_size
-    if splits is None:
-        splits = ops.decode_splits(n_rows, kv_heads, min(max_context, window + 16) if window else max_context)
-    part_o = part_m = None
-    if splits > 1:
-        n = n_rows * q_heads * splits
-        part = torch.empty(n * (head_dim + 3), dtype=torch.float32, device=q.device)
-        part_o, part_m = part[:n * head_dim], part[n * head_dim:]
+    max_pages = block_table.shape[1]
+    if blocks is None:
+        reach = min(max_context, max_pages * page_size)
+        blocks = attention_blocks(n_rows, kv_heads, q_heads // kv_heads, min(reach, window) if window else reach, ops.SM_COUNT)
+    scratch = None
+    if blocks:
+        scratch = q.new_empty((n_rows * kv_heads + blocks) * (q_heads // kv_heads) * (head_dim + 3) + n_rows + 2, dtype=torch.float32)
     ops._check(ops.lib().tllm_attention_fp8_decode(
-        ops._p(q), k, v, s, stride, ops._p(positions), ops._p(token_slot), ops._p(rows), n_rows, ops._p(block_table), block_table.shape[1], page_size,
-        q_heads, kv_heads, head_dim, int(window or 0), float(scale), splits, ops._p(part_o), ops._p(part_m), ops._p(out), ops._stream()),
-        "paged_attention_decode_fp8", kernels=2 if splits > 1 else 1)
+        q.data_ptr(), k, v, s, stride, positions.data_ptr(), token_slot.data_ptr(), None if rows is None else rows.data_ptr(), n_rows,
+        block_table.data_ptr(), max_pages, page_size, q_heads, kv_heads, head_dim, window or 0, scale, blocks,
+        None if scratch is None else scratch.data_ptr(), out.data_ptr(), ops._stream()), "paged_attention_decode_fp8", 2 if blocks else 1)
     return out
 
 
