@@ -41,6 +41,16 @@ __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t pair) {
     return d;
 }
 
+// Four at once: the low and the high half of a word.
+__device__ __forceinline__ void e4m3x4_to_half2(uint32_t word, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 l, h;\n\t"
+        "mov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}\n"
+        : "=r"(lo), "=r"(hi)
+        : "r"(word));
+}
+
 // D[16x8] += A[16x16] . B[16x8], float16 operands, float32 sums.
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
     asm volatile(

@@ -67,6 +67,14 @@ __device__ __forceinline__ float fast_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float fast_log2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void cp_async_all(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src));
+}
 // The largest (the sum) over the eight lanes that hold the same heads and other keys.
 __device__ __forceinline__ float keys_max(float v) {
 #pragma unroll
@@ -153,14 +161,22 @@ __device__ __forceinline__ void attend_run(unsigned char* smem, const A8Row& row
                 const int first = key0 + 16 * h;
                 const size_t at = (size_t)max(page[h], 0) * cache.stride, token = (size_t)g * page_size + (h == 0 ? in_page : wraps ? in_page + 16 - page_size : in_page + 16);
                 const uint8_t *kp = k0 + at + token * HD, *vp = v0 + at + token * HD;
-                const bool whole = page[h] >= 0 && first >= lo && first + 15 <= pos;
                 constexpr int kPieces = 16 * HD / 16 / 32;         // per lane: 4 or 2
+                if (page[h] >= 0 && first >= lo && first + 15 <= pos) {
 #pragma unroll
-                for (int i = 0; i < kPieces; ++i) {
-                    const int n = lane + 32 * i, row = n / (HD / 16), chunk = n % (HD / 16);
-                    const bool ok = whole || (page[h] >= 0 && first + row >= lo && first + row <= pos);
-                    cp_async_16(dst + key_dst + h * 16 * HD + i * 512, kp + i * 512, ok);
-                    cp_async_16(dst + Unit::kPlane + Unit::value_at(row, chunk) + h * 16 * HD, vp + i * 512, ok);
+                    for (int i = 0; i < kPieces; ++i) {
+                        const int n = lane + 32 * i;
+                        cp_async_all(dst + key_dst + h * 16 * HD + i * 512, kp + i * 512);
+                        cp_async_all(dst + Unit::kPlane + Unit::value_at(n / (HD / 16), n % (HD / 16)) + h * 16 * HD, vp + i * 512);
+                    }
+                } else {                                           // some of them do not count
+#pragma unroll
+                    for (int i = 0; i < kPieces; ++i) {
+                        const int n = lane + 32 * i, row = n / (HD / 16);
+                        const bool ok = page[h] >= 0 && first + row >= lo && first + row <= pos;
+                        cp_async_16(dst + key_dst + h * 16 * HD + i * 512, kp + i * 512, ok);
+                        cp_async_16(dst + Unit::kPlane + Unit::value_at(row, n % (HD / 16)) + h * 16 * HD, vp + i * 512, ok);
+                    }
                 }
                 if (lane < 8) cp_async_16(dst + 2 * Unit::kPlane + h * 128 + lane * 16, cache.scales + at + token * 8 + lane * 16, page[h] >= 0);   // masked below
             }
@@ -252,7 +268,9 @@ __device__ __forceinline__ void attend_run(unsigned char* smem, const A8Row& row
                 const uint32_t wa[4] = {ra.x, ra.y, ra.z, ra.w}, wb[4] = {rb.x, rb.y, rb.z, rb.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t a[4] = {e4m3x2_to_half2(wa[i]), e4m3x2_to_half2(wb[i]), e4m3x2_to_half2(wa[i] >> 16), e4m3x2_to_half2(wb[i] >> 16)};
+                    uint32_t a[4];
+                    e4m3x4_to_half2(wa[i], a[0], a[2]);
+                    e4m3x4_to_half2(wb[i], a[1], a[3]);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma_f16_16816(s[nt][h], a, qb[nt][4 * f + i]);
                 }
@@ -265,17 +283,25 @@ __device__ __forceinline__ void attend_run(unsigned char* smem, const A8Row& row
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const float2 sc = st[16 * h + 8 * e + gr];
-                const int j = first + 16 * h + 8 * e;
-                const bool ok = whole || (j >= lo && j <= pos);
-                lv[h][e] = ok ? __log2f(sc.y) : -INFINITY;
+                lv[h][e] = fast_log2(sc.y);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        float& x = s[nt][h][2 * e + n];
-                        x = ok ? x * (sc.x * to_score[nt][n]) : -INFINITY;
-                    }
+                    for (int n = 0; n < 2; ++n) s[nt][h][2 * e + n] *= sc.x * to_score[nt][n];
             }
+        if (!whole)                                                // keys that do not count
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int j = first + 16 * h + 8 * e;
+                    if (j >= lo && j <= pos) continue;
+                    lv[h][e] = -INFINITY;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) s[nt][h][2 * e + n] = -INFINITY;
+                }
         // ---- maxima, sums and weights, head by head
         uint32_t pb[NT][2][2];                                     // weights as the right operand: keys 2 c, + 1 (and 8 further) of sixteen h, head gr
 #pragma unroll
@@ -339,8 +365,11 @@ __device__ __forceinline__ void attend_run(unsigned char* smem, const A8Row& row
             for (int i = 0; i < kWords; ++i) {
                 const uint32_t x0 = pairs_low(vw[0][i], vw[1][i]), x1 = pairs_high(vw[0][i], vw[1][i]);
                 const uint32_t y0 = pairs_low(vw[2][i], vw[3][i]), y1 = pairs_high(vw[2][i], vw[3][i]);
-                const uint32_t a0[4] = {e4m3x2_to_half2(x0), e4m3x2_to_half2(x0 >> 16), e4m3x2_to_half2(y0), e4m3x2_to_half2(y0 >> 16)};
-                const uint32_t a1[4] = {e4m3x2_to_half2(x1), e4m3x2_to_half2(x1 >> 16), e4m3x2_to_half2(y1), e4m3x2_to_half2(y1 >> 16)};
+                uint32_t a0[4], a1[4];
+                e4m3x4_to_half2(x0, a0[0], a0[1]);
+                e4m3x4_to_half2(y0, a0[2], a0[3]);
+                e4m3x4_to_half2(x1, a1[0], a1[1]);
+                e4m3x4_to_half2(y1, a1[2], a1[3]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     mma_f16_16816(o[nt][2 * i], a0, pb[nt][h]);

@@ -200,10 +200,13 @@ fp8_skinny_kernel(const void* x, const float* sx, const uint8_t* __restrict__ w,
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t a[4] = {e4m3x2_to_half2(l[i]), e4m3x2_to_half2(h[i]), e4m3x2_to_half2(l[i] >> 16), e4m3x2_to_half2(h[i] >> 16)};
+                uint32_t a[4];
+                e4m3x4_to_half2(l[i], a[0], a[2]);
+                e4m3x4_to_half2(h[i], a[1], a[3]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    const uint32_t b[2] = {e4m3x2_to_half2(xw[nt][i]), e4m3x2_to_half2(xw[nt][i] >> 16)};
+                    uint32_t b[2];
+                    e4m3x4_to_half2(xw[nt][i], b[0], b[1]);
                     mma_f16_16816(part[nt], a, b);
                 }
             }
