@@ -37,12 +37,25 @@ def test_values_follow_the_layout_of_the_scales():
     assert gated[0, 0] == 0 and gated[8, 0] == 2 and gated[247, 0] == 0 and gated[255, 143] == 3 and gated[256, 0] == 4 and gated[264, 0] == 6
 
 
-@pytest.mark.parametrize("rows", [33, 64, 128, 129, 500, 2048, 100000])
-@pytest.mark.parametrize("n,k", [(8, 16), (1024, 128), (4096, 4096), (24576, 4096), (130, 12288)])
-def test_shares_cover_all_blocks_and_none_is_empty(rows, n, k):
-    route, splits, each = fp8._plan(rows, n, k, 148)
+@pytest.mark.parametrize("rows", [9, 16, 17, 33, 64, 128, 129, 500, 2048, 100000])
+@pytest.mark.parametrize("n,k", [(8, 16), (1024, 128), (4096, 4096), (24576, 4096), (130, 12288), (48, 2064)])
+@pytest.mark.parametrize("gated,to_float", [(False, False), (True, False), (False, True)])
+def test_shares_cover_all_blocks_and_none_is_empty(rows, n, k, gated, to_float):
+    route, splits, each = fp8._plan(rows, n, k, 148, gated, to_float)
     kb = -(-k // 128)
     assert (splits == 1 or route == fp8.TILES) and (splits - 1) * each < kb <= splits * each
+    assert route != fp8.SKINNY or rows <= 16
+    assert route != fp8.PAIRS or not to_float
+
+
+def test_scratch_holds_what_a_product_leaves_in_it():
+    # rows in 8 bits, their scales rounded up to 16 bytes, sums
+    kind, route, splits, each, size, kernels = fp8._call(61, 4096, 4096, 1, False, False, 148)
+    assert (kind, route) == (1, fp8.TILES) and size == 61 * 4096 + 61 * 32 * 4 + 4 * splits * 61 * 4096 and kernels == 3
+    assert fp8._call(8, 4096, 4096, 1, False, False, 148)[0::4] == (fp8.INSIDE, 0)
+    kind, route, splits, each, size, kernels = fp8._call(3, 512, 144, 0, True, False, 148)
+    assert (kind, route, kernels) == (0, fp8.SKINNY, 3) and size == 3 * 144 + 32 + 4 * 3 * 256
+    assert fp8._call(2048, 24576, 4096, fp8.ROWS8, True, False, 148)[1:5:3] == (fp8.PAIRS, 0)
 
 
 def test_tensors_of_the_host_are_refused():

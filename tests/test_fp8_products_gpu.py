@@ -30,7 +30,7 @@ def check_rows(got, x):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("t,k", [(1, 16), (2, 128), (3, 144), (17, 4096), (501, 1552), (0, 256)])
+@pytest.mark.parametrize("t,k", [(1, 16), (2, 128), (3, 144), (17, 4096), (501, 1552), (0, 256), (1500, 8208)])
 def test_rows(t, k, dtype):
     from tiny_llm_infer_b200 import ops
     x = rows_of(gen(t + k), t, k, dtype)

@@ -21,35 +21,44 @@ template <> __device__ __forceinline__ void load8<bf16>(const bf16* p, float (&v
     }
 }
 
-// Sixteen lanes make one block of 128: eight columns each, one 16-byte read (bfloat16), one 8-byte write.  Bound by HBM or, for
-// a few rows, by its launch.
-template <typename T>
-__global__ void __launch_bounds__(256) fp8_rows_kernel(const T* x, uint8_t* __restrict__ q, float* __restrict__ scales, int K, int kb,
-                                                       long long blocks) {
+// Sixteen lanes make one block of 128: eight columns each, one 16-byte read (bfloat16), one 8-byte write; PER blocks, all their reads on their
+// way at once.  Bound by HBM or, for a few rows, by its launch.
+template <typename T, int PER>
+__global__ void __launch_bounds__(256) fp8_rows_kernel(const T* x, uint8_t* __restrict__ q, float* __restrict__ scales, int K, unsigned kb,
+                                                       unsigned blocks) {
     TLLM_PDL_ENTER();
     const int lane16 = threadIdx.x & 15;
-    const long long b = (long long)blockIdx.x * (blockDim.x >> 4) + (threadIdx.x >> 4);
-    const long long row = b / kb;
-    const int col = (int)(b - row * kb) * kFp8Block + lane16 * 8;
-    const bool live = b < blocks && col < K;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (live) load8<T>(x + row * K + col, v);
-    const float s = fp8_scale(half_warp_max(largest8(v)));
-    const float inv = 1.0f / s;
-    if (live) *reinterpret_cast<uint2*>(q + row * K + col) = to_e4m3x8(v, inv);
-    if (lane16 == 0 && b < blocks) scales[b] = s;
+    const unsigned first = blockIdx.x * PER * (blockDim.x >> 4) + (threadIdx.x >> 4);
+    float v[PER][8];
+    long long at[PER];                                           // of the lane's columns; negative: none
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const unsigned b = first + i * (blockDim.x >> 4), row = b / kb;
+        const int col = (int)(b - row * kb) * kFp8Block + lane16 * 8;
+        at[i] = b < blocks && col < K ? (long long)row * K + col : -1;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
+        if (at[i] >= 0) load8<T>(x + at[i], v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const unsigned b = first + i * (blockDim.x >> 4);
+        const float s = fp8_scale(half_warp_max(largest8(v[i])));
+        if (at[i] >= 0) *reinterpret_cast<uint2*>(q + at[i]) = to_e4m3x8(v[i], 1.0f / s);
+        if (lane16 == 0 && b < blocks) scales[b] = s;
+    }
 }
 
 // act(gate) * up of sums that lie interleaved by eight ([rows][2 I]: eight gate, their eight up, ...), summed over `splits` shares of
 // K one after the other, as 8-bit rows.  Sixteen lanes make a block of 128 outputs, eight each, from sixteen neighbouring sums.
 __global__ void __launch_bounds__(256) fp8_gated_rows_kernel(const float* sums, int splits, long long share, uint8_t* __restrict__ q,
-                                                             float* __restrict__ scales, int inter, int ib, long long blocks, int act,
+                                                             float* __restrict__ scales, int inter, unsigned ib, unsigned blocks, int act,
                                                              GateConst gc) {
     TLLM_PDL_ENTER();
     const int lane16 = threadIdx.x & 15;
-    const long long b = (long long)blockIdx.x * (blockDim.x >> 4) + (threadIdx.x >> 4);
-    const long long row = b / ib;
-    const int col = (int)(b - row * ib) * kFp8Block + lane16 * 8;
+    const unsigned b = blockIdx.x * (blockDim.x >> 4) + (threadIdx.x >> 4), in_row = b / ib;
+    const size_t row = in_row;
+    const int col = (int)(b - in_row * ib) * kFp8Block + lane16 * 8;
     const bool live = b < blocks && col < inter;
     float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (live) {
@@ -199,11 +208,17 @@ extern "C" int tllm_fp8_rows(const void* x, int dtype, void* q, float* scales, i
     if (rows == 0) return 0;
     const int kb = (K + kFp8Block - 1) / kFp8Block;
     const long long blocks = (long long)rows * kb, grid = (blocks + 15) / 16;
-    TLLM_REQUIRE(grid <= 0x7fffffff, "fp8_rows: too many rows");
-    if (dtype == kF32)
-        launch_pdl(kPdlAlways, fp8_rows_kernel<float>, dim3((unsigned)grid), dim3(256), 0, stream, (const float*)x, (uint8_t*)q, scales, K, kb, blocks);
-    else
-        launch_pdl(kPdlAlways, fp8_rows_kernel<bf16>, dim3((unsigned)grid), dim3(256), 0, stream, (const bf16*)x, (uint8_t*)q, scales, K, kb, blocks);
+    TLLM_REQUIRE(blocks <= 0x7fffffff, "fp8_rows: too many rows");
+    // four blocks a lane once that leaves every SM four thread blocks and more
+    const bool four = grid >= 4 * 4 * 148;
+    const unsigned n = (unsigned)(four ? (blocks + 63) / 64 : grid);
+#define ROWS8(T, PER) launch_pdl(kPdlAlways, fp8_rows_kernel<T, PER>, dim3(n), dim3(256), 0, stream, (const T*)x, (uint8_t*)q, scales, K, (unsigned)kb, (unsigned)blocks)
+    if (dtype == kF32) {
+        if (four) ROWS8(float, 4); else ROWS8(float, 1);
+    } else {
+        if (four) ROWS8(bf16, 4); else ROWS8(bf16, 1);
+    }
+#undef ROWS8
     return finish_launch("fp8_rows");
 }
 
@@ -217,9 +232,9 @@ extern "C" int tllm_fp8_gated_rows(const float* sums, int splits, void* q, float
     if (rows == 0) return 0;
     const int ib = (inter + kFp8Block - 1) / kFp8Block;
     const long long blocks = (long long)rows * ib, grid = (blocks + 15) / 16;
-    TLLM_REQUIRE(grid <= 0x7fffffff, "fp8_gated_rows: too many rows");
+    TLLM_REQUIRE(blocks <= 0x7fffffff, "fp8_gated_rows: too many rows");
     launch_pdl(kPdlAlways, fp8_gated_rows_kernel, dim3((unsigned)grid), dim3(256), 0, stream, sums, splits, (long long)rows * inter * 2,
-               (uint8_t*)q, scales, inter, ib, blocks, act, GateConst{limit, slope});
+               (uint8_t*)q, scales, inter, (unsigned)ib, (unsigned)blocks, act, GateConst{limit, slope});
     return finish_launch("fp8_gated_rows");
 }
 

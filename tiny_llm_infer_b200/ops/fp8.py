@@ -221,21 +221,39 @@ def add_rmsnorm_fp8(h: torch.Tensor, delta: Optional[torch.Tensor], gain: torch.
     return out
 
 
-SKINNY_ROWS = 16         # up to this many rows the weight-streaming kernel
+SKINNY_ROWS = 8          # up to this many rows always the weight-streaming kernel,
+SKINNY_WIDE_ROWS = 16    # and up to this many where it is ahead of the tensor cores' kernels
 SKINNY_INSIDE_K = 4096   # up to this many columns it rounds eight bfloat16 rows itself
 SKINNY, TILES, PAIRS = 0, 1, 2           # routes of csrc/fp8_product.cu
 ROWS8, INSIDE = 2, 3                     # kinds of rows there, beside float32 and bfloat16
 
 
-def _plan(rows: int, n: int, k: int, sms: int):
-    """(route, shares of K, blocks per share) of a product with ``n`` weight rows on the tensor cores."""
+def _plan(rows: int, n: int, k: int, sms: int, gated: bool = False, to_float: bool = False):
+    """(route, shares of K, blocks per share) of a product with ``n`` weight rows, by what the kernels take, in us.  Tiles of 128 x 128:
+    4 and, for every round of tiles, 0.7 and 0.37 a block of K; more than one share, and gated products, leave float32 sums for another kernel:
+    1 and their bytes twice at 8 TB/s.  Tiles of 256 x 256 by pairs of SMs: 3 and, a round, 1 and 0.47 a block.  Nine to sixteen rows by the
+    weight-streaming kernel: 2.5 and the weight's bytes at 3 TB/s.  (Measured and by this rule, rows x columns x K: 61 x 4096 x 4096 in 4 shares 9.5
+    and 9.7, in one 14.5 and 16.5, in 5 (two rounds) 12.3 and 12.8; 128 in 4 10.4 and 10.8, 17 in 4 9.2 and 8.9; 61 x 4096 x 12288 in 4 16.2 and
+    15.6; 61 x 24576 x 4096 in one share 29 both; 300 x 4096 x 4096 tiles 14.9 and 16.5, pairs 18.0 and 19.0; 1200 x 4096 x 4096 pairs 33 and 35,
+    tiles 40 and 42; 16 x 24576 x 4096 streaming 37 and 36, 16 x 4096 x 4096 8.0 both.)"""
     kb = _blocks(k)
-    if -(-rows // 256) * -(-n // 256) >= sms // 4:
-        return PAIRS, 1, kb
     tiles = _blocks(rows) * _blocks(n)
-    splits = max(1, min(sms // tiles, kb // 2))
-    each = -(-kb // splits)
-    return TILES, -(-kb // each), each
+    best = None
+    for splits in range(1, max(1, min(16, kb // 2)) + 1):
+        each = -(-kb // splits)
+        used = -(-kb // each)
+        us = 4 + -(-tiles * used // sms) * (0.7 + 0.37 * each)
+        if used > 1 or gated or to_float:
+            us += 1 + 8 * used * rows * n / 8e6
+        if best is None or us < best[0]:
+            best = (us, TILES, used, each)
+    if not to_float:                             # pairs write bfloat16 or, gated, 8 bits
+        us = 3 + -(-(-(-rows // 256) * -(-n // 256)) // (sms // 2)) * (1 + 0.47 * kb)
+        if us < best[0]:
+            best = (us, PAIRS, 1, kb)
+    if rows <= SKINNY_WIDE_ROWS and 2.5 + n * k / 3e6 < best[0]:
+        best = (0, SKINNY, 1, kb)
+    return best[1:]
 
 
 @functools.lru_cache(maxsize=8192)
@@ -246,9 +264,7 @@ def _call(rows: int, n: int, k: int, kind: int, gated: bool, to_float: bool, sms
         if kind == 1 and rows <= 8 and k <= SKINNY_INSIDE_K:
             kind = INSIDE
     else:
-        route, splits, each = _plan(rows, n, k, sms)
-        if route == PAIRS and to_float:          # pairs write bfloat16 or, gated, 8 bits
-            route = TILES
+        route, splits, each = _plan(rows, n, k, sms, gated, to_float)
     scratch = 0 if kind in (ROWS8, INSIDE) else rows * k + -(-4 * rows * _blocks(k) // 16) * 16
     kernels = 1 + (kind not in (ROWS8, INSIDE))
     if gated:
