@@ -125,3 +125,10 @@ def test_pages_of_portions():
     assert fp8.portion_pages(ctx, 16, 20, 40) == (4, 1 + 2 + 4)      # from the page of 81 to that of 132
     assert fp8.portion_pages(SimpleNamespace(segments=[seg(5, 1)]), 16, None, 40) == (1, 1)
     assert fp8.portion_pages(ctx, 16, 20, 40, capturing=True) == (40, 120)
+
+
+def test_few_keys_have_a_block_of_their_own_and_many_are_shared():
+    blocks = fp8.attention_blocks
+    assert blocks(1, 8, 4, 64, 148) == blocks(16, 8, 2, 600, 148) == blocks(24, 8, 2, 1000, 148) == blocks(0, 8, 4, 9999, 148) == 0
+    assert blocks(1, 8, 4, 1000, 148) == blocks(64, 8, 4, 4096, 148) == 444 and blocks(2, 1, 16, 100000, 148) == 296
+    assert blocks(513, 8, 4, 100000, 148) == 0

@@ -476,23 +476,17 @@ template <int HD, int NT>
 __global__ void __launch_bounds__(kA8Warps * 32, NT == 1 ? 3 : 2)
 attention_fp8_share_kernel(const A8Step st, int* __restrict__ plan, float* __restrict__ part_o, float* __restrict__ part_m, bf16* __restrict__ out) {
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int before[kA8MaxRows + 1], sums[2][kA8Warps];
+    __shared__ int before[kA8MaxRows + 1], units[kA8MaxRows], sums[2][kA8Warps];
     TLLM_PDL_ENTER();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = st.q_heads / st.kv_heads, blocks = gridDim.x;
-    // units of four rows a thread; sums over the block
-    constexpr int kEach = kA8MaxRows / (kA8Warps * 32);
-    int units[kEach], some = 0, rows_here = 0;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        const int ridx = threadIdx.x * kEach + i;
-        units[i] = 0;
-        if (ridx < st.n_rows) {
-            const int r = st.rows ? st.rows[ridx] : ridx;
-            const int pos = st.positions[r];
-            if (st.token_slot[r] >= 0) units[i] = units_of(pos, st.window);
-        }
-        some += units[i];
-        rows_here += units[i] > 0;
+    int some = 0, rows_here = 0;
+    for (int ridx = threadIdx.x; ridx < st.n_rows; ridx += kA8Warps * 32) {
+        const int r = st.rows ? st.rows[ridx] : ridx;
+        const int pos = st.positions[r], slot = st.token_slot[r];
+        const int n = slot >= 0 ? units_of(pos, st.window) : 0;
+        units[ridx] = n;                                           // read back by this thread alone
+        some += n;
+        rows_here += n > 0;
     }
     int turn = 0;
     auto block_total = [&](int v) {
@@ -513,36 +507,33 @@ attention_fp8_share_kernel(const A8Step st, int* __restrict__ plan, float* __res
         // the shortest of a few lengths, a sixteenth longer each time: with twice as many blocks as pairs, twice the mean length always does
         for (;;) {
             int c = 0;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) c += (units[i] + each - 1) / each;
+            for (int ridx = threadIdx.x; ridx < st.n_rows; ridx += kA8Warps * 32) c += (units[ridx] + each - 1) / each;
             if (block_total(c) * st.kv_heads <= blocks) break;
             each += max(each / 16 / kA8Warps, 1) * kA8Warps;
         }
     }
     // chunks or units of a head before each row
-    int mine[kEach], run = 0;
+    int all = 0;
+    for (int first = 0; first < st.n_rows; first += kA8Warps * 32) {
+        const int ridx = first + threadIdx.x;
+        const int n = ridx < st.n_rows ? (chunks ? (units[ridx] + each - 1) / each : units[ridx]) : 0;
+        int upto = n;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        mine[i] = run;
-        run += chunks ? (units[i] + each - 1) / each : units[i];
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        if (lane == 31) sums[turn][warp] = upto;
+        __syncthreads();
+        int offset = all + upto - n;
+#pragma unroll
+        for (int i = 0; i < kA8Warps; ++i) {
+            if (i < warp) offset += sums[turn][i];
+            all += sums[turn][i];
+        }
+        turn ^= 1;
+        if (ridx < st.n_rows) before[ridx] = offset;
     }
-    int upto = run;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
-    }
-    if (lane == 31) sums[turn][warp] = upto;
-    __syncthreads();
-    int offset = upto - run, all = 0;
-#pragma unroll
-    for (int i = 0; i < kA8Warps; ++i) {
-        if (i < warp) offset += sums[turn][i];
-        all += sums[turn][i];
-    }
-#pragma unroll
-    for (int i = 0; i < kEach; ++i)
-        if (threadIdx.x * kEach + i < st.n_rows) before[threadIdx.x * kEach + i] = offset + mine[i];
     if (threadIdx.x == 0) before[st.n_rows] = all;
     __syncthreads();
     if (blockIdx.x == 0) {
@@ -556,7 +547,7 @@ attention_fp8_share_kernel(const A8Step st, int* __restrict__ plan, float* __res
     const int end = chunks ? at + 1 : min(at + each, here);
     // the row that holds it: the last one with before * kv_heads <= at (rows with nothing are passed over)
     int ridx = 0;
-    for (int step = kA8MaxRows / 2; step > 0; step >>= 1)
+    for (int step = st.n_rows > 64 ? kA8MaxRows / 2 : 32; step > 0; step >>= 1)
         if (ridx + step < st.n_rows && before[ridx + step] * st.kv_heads <= at) ridx += step;
     while (at < end) {
         const int n = before[ridx + 1] - before[ridx];
@@ -598,7 +589,7 @@ attention_fp8_join_kernel(const A8Step st, const int* plan, const float* part_o,
     constexpr int kDims = HD / 32;
     __shared__ float sums[WIDE ? kA8JoinWarps : 1][HD];
     TLLM_PDL_ENTER();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5, ridx = blockIdx.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5, ridx = blockIdx.y;       // WIDE: kA8JoinWarps warps
     const int r = st.rows ? st.rows[ridx] : ridx, group = st.q_heads / st.kv_heads, slot = st.token_slot[r];
     const int before = plan[ridx], n = plan[ridx + 1] - before, each = plan[st.n_rows + 1];
     const int g = WIDE ? blockIdx.x / group : blockIdx.x;
@@ -617,28 +608,51 @@ attention_fp8_join_kernel(const A8Step st, const int* plan, const float* part_o,
         const size_t base = ((each == 0 ? (size_t)0 : (size_t)ridx * st.kv_heads + g) + b0) * group + h;      // the first piece's place
         const float* me = part_m + base * 3;
         const float* oe = part_o + base * HD + lane * kDims;
-        float mm = -INFINITY, dn = -INFINITY, total = 0.0f;
-        for (int p = lane; p < pieces; p += 32) mm = fmaxf(mm, me[p * group * 3]);
+        // the first pieces' numbers and values, all on their way at once
+        constexpr int kAhead = 4, kApart = WIDE ? kA8JoinWarps : 1;
+        const int mine = WIDE ? warp : 0;
+        const bool there = lane < pieces;
+        const float m0 = there ? me[lane * group * 3] : -INFINITY, d0 = there ? me[lane * group * 3 + 1] : -INFINITY;
+        const float l0 = there ? me[lane * group * 3 + 2] : 0.0f;
+        float ahead[kAhead][kDims];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+            for (int e = 0; e < kDims; ++e) ahead[i][e] = mine + i * kApart < pieces ? oe[(size_t)(mine + i * kApart) * group * HD + e] : 0.0f;
+        float mm = m0, dn = -INFINITY, total = 0.0f;
+        for (int p = lane + 32; p < pieces; p += 32) mm = fmaxf(mm, me[p * group * 3]);
         mm = warp_max(mm);
         // a piece without keys has M of -infinity and sums of zero; scores that are all NaN leave M so too, and l NaN
-        for (int p = lane; p < pieces; p += 32) {
-            const float m = me[p * group * 3], l = me[p * group * 3 + 2];
+        auto take = [&](float m, float d, float l) {
             total += m == -INFINITY ? l : l * exp2f(m - mm);
-            if (m != -INFINITY) dn = fmaxf(dn, me[p * group * 3 + 1] + (m - mm));
-        }
+            if (m != -INFINITY) dn = fmaxf(dn, d + (m - mm));
+        };
+        take(m0, d0, l0);
+        for (int p = lane + 32; p < pieces; p += 32) take(me[p * group * 3], me[p * group * 3 + 1], me[p * group * 3 + 2]);
         dn = warp_max(dn);
         total = warp_sum(total);
+        auto factor_of = [&](float m, float d) {
+            const float of = m == -INFINITY ? -INFINITY : d + (m - mm);
+            return of == -INFINITY ? 0.0f : exp2f(of - dn);
+        };
         float acc[kDims];
 #pragma unroll
         for (int i = 0; i < kDims; ++i) acc[i] = 0.0f;
-        for (int p0 = 0; p0 < pieces; p0 += 32) {
-            const int p = p0 + lane;
-            const float m = p < pieces ? me[p * group * 3] : -INFINITY;
-            const float of = m == -INFINITY ? -INFINITY : me[p * group * 3 + 1] + (m - mm);
-            const float factor = of == -INFINITY ? 0.0f : exp2f(of - dn);
+        float factor = factor_of(m0, d0);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const float f = __shfl_sync(0xffffffffu, factor, mine + i * kApart);                 // at most piece 31
+#pragma unroll
+            for (int e = 0; e < kDims; ++e) acc[e] = fmaf(ahead[i][e], f, acc[e]);
+        }
+        for (int p0 = 0, from = mine + kAhead * kApart; p0 < pieces; p0 += 32, from = mine) {
+            if (p0 > 0) {
+                const int p = p0 + lane;
+                factor = p < pieces ? factor_of(me[p * group * 3], me[p * group * 3 + 1]) : 0.0f;
+            }
             const int count = min(32, pieces - p0);
 #pragma unroll 4
-            for (int i = WIDE ? warp : 0; i < count; i += WIDE ? warps : 1) {
+            for (int i = from; i < count; i += kApart) {
                 const float f = __shfl_sync(0xffffffffu, factor, i);
                 const float* o = oe + (size_t)(p0 + i) * group * HD;
 #pragma unroll
@@ -674,18 +688,18 @@ static int launch_attention_fp8(const A8Step& st, int blocks, int* plan, float* 
         configured.done();
     }
     if (blocks == 0) {
-        launch_pdl(kPdlAlways, attention_fp8_whole_kernel<HD, NT>, dim3(st.kv_heads, st.n_rows), dim3(kA8Warps * 32), smem, stream, st, (bf16*)out);
+        launch_pdl(kPdlAttention, attention_fp8_whole_kernel<HD, NT>, dim3(st.kv_heads, st.n_rows), dim3(kA8Warps * 32), smem, stream, st, (bf16*)out);
         return finish_launch("attention_fp8_whole");
     }
-    launch_pdl(kPdlAlways, attention_fp8_share_kernel<HD, NT>, dim3(blocks), dim3(kA8Warps * 32), smem, stream, st, plan, part_o, part_m, (bf16*)out);
+    launch_pdl(kPdlAttention, attention_fp8_share_kernel<HD, NT>, dim3(blocks), dim3(kA8Warps * 32), smem, stream, st, plan, part_o, part_m, (bf16*)out);
     const int rc = finish_launch("attention_fp8_share");
     if (rc != 0) return rc;
     const int group = st.q_heads / st.kv_heads;
     if ((long long)st.n_rows * st.kv_heads * 8 <= blocks)         // eight pieces a head and more, on average
-        launch_pdl(kPdlAlways, attention_fp8_join_kernel<HD, true>, dim3(st.q_heads, st.n_rows), dim3(kA8JoinWarps * 32), 0, stream, st,
+        launch_pdl(kPdlCombine, attention_fp8_join_kernel<HD, true>, dim3(st.q_heads, st.n_rows), dim3(kA8JoinWarps * 32), 0, stream, st,
                    (const int*)plan, (const float*)part_o, (const float*)part_m, (bf16*)out);
     else
-        launch_pdl(kPdlAlways, attention_fp8_join_kernel<HD, false>, dim3(st.kv_heads, st.n_rows), dim3((group < kA8JoinWarps ? group : kA8JoinWarps) * 32),
+        launch_pdl(kPdlCombine, attention_fp8_join_kernel<HD, false>, dim3(st.kv_heads, st.n_rows), dim3((group < kA8JoinWarps ? group : kA8JoinWarps) * 32),
                    0, stream, st, (const int*)plan, (const float*)part_o, (const float*)part_m, (bf16*)out);
     return finish_launch("attention_fp8_join");
 }
@@ -801,10 +815,10 @@ extern "C" int tllm_attention_fp8_unpack(const void* k, const void* v, const voi
     TLLM_REQUIRE((long long)2 * kv_heads * page_size * (head_dim / 16) <= 0x7fffffff, "attention_fp8_unpack: too large");
     const A8Cache cache{(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)scales, page_bytes};
     if (head_dim == 64)
-        launch_pdl(kPdlAlways, attention_fp8_unpack_kernel<64>, dim3(per, segments), dim3(256), 0, stream, cache, seg_info, block_table, max_pages,
+        launch_pdl(kPdlOther, attention_fp8_unpack_kernel<64>, dim3(per, segments), dim3(256), 0, stream, cache, seg_info, block_table, max_pages,
                    page_size, kv_heads, window, capacity, (bf16*)pages, table);
     else
-        launch_pdl(kPdlAlways, attention_fp8_unpack_kernel<128>, dim3(per, segments), dim3(256), 0, stream, cache, seg_info, block_table, max_pages,
+        launch_pdl(kPdlOther, attention_fp8_unpack_kernel<128>, dim3(per, segments), dim3(256), 0, stream, cache, seg_info, block_table, max_pages,
                    page_size, kv_heads, window, capacity, (bf16*)pages, table);
     return finish_launch("attention_fp8_unpack");
 }

@@ -428,16 +428,21 @@ def _attention_operands(what, q, out, positions, token_slot, rows, n_rows, block
         _refuse(f"{what}: {n_rows} rows of {shape[0]}, a position and a slot for each")
 
 
-SHARED_ROWS = 512        # at most so many rows share blocks
-SHARED_FROM = 512        # and only where a row may see more keys than this
+SHARED_ROWS = 512        # rows that may share blocks
 
 
 def attention_blocks(rows: int, kv_heads: int, group: int, reach: int, sms: int) -> int:
-    """Blocks of threads that share all rows' keys in ``paged_attention_decode_fp8``, or 0 for one block per (row, key/value head) and no
-    second kernel."""
-    if rows > SHARED_ROWS or reach <= SHARED_FROM:
+    """Blocks of threads that share all rows' keys in ``paged_attention_decode_fp8`` (as many as are resident at once), or 0 for one block
+    per (row, key/value head) and no second kernel: whichever should take less.  A block of its own takes 3.5 us and 1.2 for every 128 of the
+    ``reach`` keys a row may see, more where the blocks are not all resident; shares take 10 us and 2.4 for every 32 keys that a warp gets, rows being
+    0.7 of the reach on average.  (us, own block and shares, rows x heads, reach: 1 x 8, 1000 11.5 and 9.0; 1 x 8, 4095 36 and 11; 8 x 8, 2000 25
+    and 16; 8 x 8, 4096 45 and 22; 64 x 8, 4096 83 and 73; 16 x 8, 600 10.6 and 12.7; 24 x 8 of width 64, 1000 13.1 and 14.9.)"""
+    if rows > SHARED_ROWS or rows == 0:
         return 0
-    return (3 if group <= 8 else 2) * sms                    # what is resident at once
+    resident, pairs = (3 if group <= 8 else 2) * sms, rows * kv_heads
+    own = 3.5 + 1.2 * reach / 128 * max(1.0, pairs / resident)
+    shared = 10 + 2.4 * max(1.0, 0.7 * pairs * reach / 32 / (4 * resident))
+    return resident if shared < own else 0
 
 
 def paged_attention_decode_fp8(q, planes, positions, token_slot, rows, n_rows, block_table, page_size, q_heads, kv_heads, head_dim, window, scale,
