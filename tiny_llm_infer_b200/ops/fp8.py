@@ -434,13 +434,13 @@ SHARED_ROWS = 512        # rows that may share blocks
 def attention_blocks(rows: int, kv_heads: int, group: int, reach: int, sms: int) -> int:
     """Blocks of threads that share all rows' keys in ``paged_attention_decode_fp8`` (as many as are resident at once), or 0 for one block
     per (row, key/value head) and no second kernel: whichever should take less.  A block of its own takes 3.5 us and 1.2 for every 128 of the
-    ``reach`` keys a row may see, more where the blocks are not all resident; shares take 10 us and 2.4 for every 32 keys that a warp gets, rows being
+    ``reach`` keys a row may see, nearly twice that where the resident blocks share HBM; shares take 10 us and 2.4 for every 32 keys that a warp gets, rows being
     0.7 of the reach on average.  (us, own block and shares, rows x heads, reach: 1 x 8, 1000 11.5 and 9.0; 1 x 8, 4095 36 and 11; 8 x 8, 2000 25
     and 16; 8 x 8, 4096 45 and 22; 64 x 8, 4096 83 and 73; 16 x 8, 600 10.6 and 12.7; 24 x 8 of width 64, 1000 13.1 and 14.9.)"""
     if rows > SHARED_ROWS or rows == 0:
         return 0
     resident, pairs = (3 if group <= 8 else 2) * sms, rows * kv_heads
-    own = 3.5 + 1.2 * reach / 128 * max(1.0, pairs / resident)
+    own = 3.5 + 1.2 * reach / 128 * max(1.0, 1.9 * pairs / resident)
     shared = 10 + 2.4 * max(1.0, 0.7 * pairs * reach / 32 / (4 * resident))
     return resident if shared < own else 0
 
