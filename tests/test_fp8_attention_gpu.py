@@ -359,3 +359,48 @@ def test_refusals():
         with pytest.raises(ops.KernelError):
             ops.qk_norm_rope_store_fp8(kw.get("qkv", qkv), None, None, 1.0, kw.get("inv"), kw.get("rot", 0), one, one, table, planes, 16, q.clone(), 4, 2, 64,
                                        kw.get("flags", 0) | ops.QK_STORE | ops.QK_QOUT)
+
+
+@pytest.mark.parametrize("blocks", [0, 30])
+def test_a_position_past_the_block_table_reads_no_other_memory(blocks):
+    """The last key that the table has room for is as far as a row sees."""
+    from tiny_llm_infer_b200 import ops
+    g = gen(13)
+    planes = planes_of(4, 2, 16, 64)
+    table = tables(g, [64], 16, 4, 4)
+    fill(g, planes, table, [64], 16, (0.3, 0.3))
+    q = torch.randn((1, 4 * 64), generator=g, device="cuda").to(torch.bfloat16)
+    outs = []
+    for pos in (63, 64, 100000):
+        outs.append(torch.empty_like(q))
+        ops.paged_attention_decode_fp8(q, planes, torch.tensor([pos], dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda"),
+                                       None, 1, table, 16, 4, 2, 64, None, 0.125, outs[-1], 64, blocks)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+def test_many_rows_of_a_step():
+    """More rows than share blocks, and as many as do: every row as if it were alone, rows of no request between them."""
+    from tiny_llm_infer_b200 import ops
+    g = gen(17)
+    q_heads, kv_heads, dim, page = 4, 2, 64, 16
+    lengths = [1 + (37 * i) % 700 for i in range(40)]
+    pages = sum(-(-n // page) for n in lengths)
+    planes = planes_of(pages, kv_heads, page, dim)
+    table = tables(g, lengths, page, pages, 44)
+    fill(g, planes, table, lengths, page, (0.3, 0.3))
+    for total, blocks in ((512, 444), (512, 1), (700, 0), (700, None), (129, 512)):
+        slots = torch.tensor([-1 if i % 7 == 3 else (i * 11) % 40 for i in range(total)], dtype=torch.int32, device="cuda")
+        pos = torch.tensor([lengths[(i * 11) % 40] - 1 for i in range(total)], dtype=torch.int32, device="cuda")
+        q = torch.randn((total, q_heads * dim), generator=g, device="cuda").to(torch.bfloat16)
+        out = torch.empty_like(q)
+        ops.paged_attention_decode_fp8(q, planes, pos, slots, None, total, table, page, q_heads, kv_heads, dim, None, 0.125, out, 700, blocks)
+        assert (out[slots < 0] == 0).all()
+        for i in (0, 1, 5, total // 2, total - 1):
+            if i % 7 == 3:
+                continue
+            r = (i * 11) % 40
+            keys, values = stored(planes, table, r, lengths[r], page)
+            want, off = exact_row(q[i].double().view(q_heads, dim), keys, values, lengths[r] - 1, 0, 0.125)
+            assert ((out[i].double() - want).abs() <= off).all()
+    with pytest.raises(ops.KernelError):
+        ops.paged_attention_decode_fp8(q, planes, pos, slots, None, 129, table, page, q_heads, kv_heads, dim, None, 0.125, out, 700, 513)

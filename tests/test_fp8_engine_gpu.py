@@ -205,3 +205,18 @@ def test_refusals(folders, tmp_path):
     for kw in (dict(quantization="fp8"), dict(kv_cache_dtype="fp8")):
         with pytest.raises(ValueError):
             LLM(str(odd), max_model_len=64, num_kv_blocks=8, **kw)
+
+
+def test_a_loaded_model_keeps_its_form(folders):
+    from tiny_llm_infer_b200 import LLM, SamplingParams
+    from tiny_llm_infer_b200.engine import load_model
+    folder, _ = folders["E"]
+    loaded = load_model(str(folder), torch.bfloat16, "cuda:0", "fp8")
+    with pytest.raises(ValueError, match="already"):
+        loaded[0].use_fp8_weights()
+    first = LLM("", loaded=loaded, max_model_len=64, num_kv_blocks=8, kv_cache_dtype="fp8")
+    with pytest.raises(ValueError, match="keeps its cache"):
+        LLM("", loaded=loaded, max_model_len=64, num_kv_blocks=8)
+    second = LLM("", loaded=loaded, max_model_len=64, num_kv_blocks=8, kv_cache_dtype="fp8")
+    params = SamplingParams(max_tokens=4, ignore_eos=True)
+    assert first.generate([[1, 2, 3]], params)[0].token_ids == second.generate([[1, 2, 3]], params)[0].token_ids

@@ -416,11 +416,14 @@ __device__ __forceinline__ void run_sums(const unsigned char* smem, int row, int
 __device__ __forceinline__ int first_key(int pos, int window) { return window > 0 && pos - window + 1 > 0 ? pos - window + 1 : 0; }
 __device__ __forceinline__ int units_of(int pos, int window) { return (pos - first_key(pos, window) / 16 * 16) / kA8Unit + 1; }
 
+// A row's position, held within what its row of the block table has room for: a caller's mistake reads no other memory.
+__device__ __forceinline__ int position_of(const int* positions, int r, int room) { return min(positions[r], room - 1); }
+
 struct A8Step {
     const bf16* q;
     A8Cache cache;
     const int *positions, *token_slot, *rows, *block_table;
-    int n_rows, max_pages, page_size, q_heads, kv_heads, window;
+    int n_rows, max_pages, page_size, q_heads, kv_heads, window, room;      // room: max_pages * page_size
     float scale_log2e;
 };
 template <int HD>
@@ -432,7 +435,7 @@ __device__ __forceinline__ A8Row row_at(const A8Step& st, int r, int slot, int g
     x.table = st.block_table + (size_t)slot * st.max_pages;
     x.page_size = st.page_size;
     x.kv_heads = st.kv_heads;
-    x.pos = st.positions[r];
+    x.pos = position_of(st.positions, r, st.room);
     x.lo = first_key(x.pos, st.window);
     x.base = x.lo / 16 * 16;
     x.scale_log2e = st.scale_log2e;
@@ -482,7 +485,7 @@ attention_fp8_share_kernel(const A8Step st, int* __restrict__ plan, float* __res
     int some = 0, rows_here = 0;
     for (int ridx = threadIdx.x; ridx < st.n_rows; ridx += kA8Warps * 32) {
         const int r = st.rows ? st.rows[ridx] : ridx;
-        const int pos = st.positions[r], slot = st.token_slot[r];
+        const int pos = position_of(st.positions, r, st.room), slot = st.token_slot[r];
         const int n = slot >= 0 ? units_of(pos, st.window) : 0;
         units[ridx] = n;                                           // read back by this thread alone
         some += n;
@@ -780,7 +783,8 @@ extern "C" int tllm_attention_fp8_decode(const void* q, const void* k, const voi
     if (check_a8("attention_fp8_decode", k, v, scales, page_bytes, page_size, kv_heads, head_dim) != 0) return -1;
     TLLM_REQUIRE(q_heads > 0 && q_heads % kv_heads == 0 && q_heads / kv_heads <= 16,
                  "attention_fp8_decode: %d query heads over %d key/value heads (at most 16 per group)", q_heads, kv_heads);
-    TLLM_REQUIRE(n_rows >= 0 && n_rows <= 65535 && q_heads <= 65535 && max_pages > 0 && window >= 0, "attention_fp8_decode: bad grid");
+    TLLM_REQUIRE(n_rows >= 0 && n_rows <= 65535 && q_heads <= 65535 && max_pages > 0 && window >= 0 && (long long)max_pages * page_size <= 0x7fffffff,
+                 "attention_fp8_decode: bad grid");
     TLLM_REQUIRE(blocks >= 0 && blocks <= kA8MaxShares && (blocks == 0 || (n_rows <= kA8MaxRows && scratch)),
                  "attention_fp8_decode: %d rows shared by %d blocks (at most 512 and 512, with scratch)", n_rows, blocks);
     TLLM_REQUIRE(blocks == 0 || (long long)n_rows * kv_heads * ((long long)max_pages * page_size / kA8Unit + 1) < 0x7fffffff - (1 << 13),
@@ -789,7 +793,7 @@ extern "C" int tllm_attention_fp8_decode(const void* q, const void* k, const voi
                  "attention_fp8_decode: missing or unaligned operands");
     if (n_rows == 0) return 0;
     const A8Step st{(const bf16*)q, A8Cache{(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)scales, page_bytes}, positions, token_slot, rows,
-                    block_table, n_rows, max_pages, page_size, q_heads, kv_heads, window, scale * 1.4426950408889634f};
+                    block_table, n_rows, max_pages, page_size, q_heads, kv_heads, window, max_pages * page_size, scale * 1.4426950408889634f};
     const int group = q_heads / kv_heads;
     const size_t places = ((size_t)n_rows * kv_heads + blocks) * group;
     float *part_o = scratch, *part_m = scratch + places * head_dim;

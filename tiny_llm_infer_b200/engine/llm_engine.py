@@ -300,7 +300,7 @@ class LLM:
     ``quantization`` "fp8": the layers' matrices are kept in 8 bits (e4m3, a float32 scale per block of 128 x 128) and meet rows rounded
     to 8 bits per 128 columns; embedding, norms and head stay in bfloat16.  ``kv_cache_dtype`` "fp8": keys and values are kept in
     8 bits, a float32 scale per token and head, half the memory and half the reading.  Both are for bfloat16 models of the
-    architectures whose parts have the form (Qwen3); others are refused.
+    architectures whose parts have the form (Qwen3); others are refused.  A model given as ``loaded`` keeps the form from then on.
     """
 
     def __init__(self, model: str, dtype: str = "bfloat16", max_model_len: int = 2048,
@@ -320,6 +320,8 @@ class LLM:
         max_model_len = min(int(max_model_len), self.model.desc.max_positions)
         block_size = min(int(block_size), max_model_len)
         cache_dtype = torch_dtype
+        if kv_cache_dtype == "auto" and self.model.fp8_cache:
+            raise ValueError("the loaded model keeps its cache in 8 bits: kv_cache_dtype='fp8'")
         if kv_cache_dtype == "fp8":
             self.model.use_fp8_cache(block_size)
             cache_dtype = torch.uint8

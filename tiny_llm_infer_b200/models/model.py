@@ -72,6 +72,7 @@ class Model:
         # (layer, one cache id per mixer of its block, writes)
         self.order = desc.resolved_order([len(b.mixers()) for b in self.blocks])
         self.loaded = False
+        self.fp8_weights = self.fp8_cache = False
 
     # ---- weights
     def load(self, tensors: Dict[str, torch.Tensor]) -> None:
@@ -93,17 +94,21 @@ class Model:
             raise ValueError("weights are brought to 8 bits after they are loaded")
         if self.dtype != torch.bfloat16:
             raise ValueError(f"8-bit weights are for bfloat16 models, this one is {self.dtype}")
+        if self.fp8_weights:
+            raise ValueError("the model's weights are in 8 bits already")
         for block in self.blocks:
             block.use_fp8_weights()
+        self.fp8_weights = True
 
     def use_fp8_cache(self, page_size: int) -> None:
-        """Keep keys and values in 8 bits; the cache manager is then made with ``dtype=torch.uint8``."""
+        """Keep keys and values in 8 bits, from here on; cache managers for the model are then made with ``dtype=torch.uint8``."""
         mixers = [m for b in self.blocks for m in b.mixers()]
         for mixer in mixers:
             if not hasattr(mixer, "use_fp8_cache"):
                 raise ValueError(f"{type(mixer).__name__} has no 8-bit cache")
         for mixer in mixers:
             mixer.use_fp8_cache(page_size)
+        self.fp8_cache = True
 
     # ---- what the cache manager must provide, per cache id
     def cache_needs(self) -> Dict[int, Tuple[Optional[CacheSpec], Optional[StateSpec]]]:
