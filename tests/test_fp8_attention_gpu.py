@@ -404,3 +404,56 @@ def test_many_rows_of_a_step():
             assert ((out[i].double() - want).abs() <= off).all()
     with pytest.raises(ops.KernelError):
         ops.paged_attention_decode_fp8(q, planes, pos, slots, None, 129, table, page, q_heads, kv_heads, dim, None, 0.125, out, 700, 513)
+
+
+@pytest.mark.parametrize("blocks", [0, 30])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_what_no_page_holds_does_not_count(dim, blocks):
+    """Entries of the table without a page, or with one the cache does not have: their keys are left out, in the middle, at either end and
+    everywhere; slots and positions of no request give zeros."""
+    from tiny_llm_infer_b200 import ops
+    g = gen(19)
+    q_heads, kv_heads, page, length = 8, 2, 16, 400
+    planes = planes_of(25, kv_heads, page, dim)
+    table = tables(g, [length] * 1, page, 25, 25)
+    fill(g, planes, table, [length], page, (0.3, 0.3))
+    keys, values = stored(planes, table, 0, length, page)
+    gone = [[], [3, 4, 11], [0], [24], [0, 1, 2, 22, 23, 24], list(range(25)), [24], []]
+    tabs = table.repeat(len(gone), 1)
+    for r, pages in enumerate(gone):
+        tabs[r, pages] = torch.tensor([-1 if i % 2 else 25 + 1000 * r for i in range(len(pages))], dtype=torch.int32, device="cuda")
+    n = len(gone)
+    pos = torch.tensor([length - 1] * (n - 2) + [385, -5], dtype=torch.int32, device="cuda")
+    slots = torch.tensor(list(range(n - 1)) + [n - 1], dtype=torch.int32, device="cuda")
+    q = torch.randn((n + 1, q_heads * dim), generator=g, device="cuda").to(torch.bfloat16)
+    pos, slots = torch.cat([pos, pos[:1]]), torch.cat([slots, slots[-1:] + 1])          # and a slot behind the table
+    out = torch.empty_like(q)
+    ops.paged_attention_decode_fp8(q, planes, pos, slots, None, n + 1, tabs, page, q_heads, kv_heads, dim, None, 0.125, out, length, blocks)
+    for r in range(n + 1):
+        left = [j for j in range(pos[r] + 1) if r < n - 1 and j // page not in gone[r]]
+        if not left:
+            assert (out[r] == 0).all()
+            continue
+        want, off = exact_row(q[r].double().view(q_heads, dim), keys[:, left], values[:, left], len(left) - 1, 0, 0.125)
+        assert ((out[r].double() - want).abs() <= off).all()
+
+
+def test_a_store_outside_the_cache_is_left_out():
+    """Positions behind the table's room, slots it does not have and pages the cache does not have: nothing is written for them."""
+    from tiny_llm_infer_b200 import ops
+    q_heads, kv_heads, dim, page = 4, 2, 64, 16
+    planes = planes_of(3, kv_heads, page, dim)
+    for plane in planes:
+        plane.fill_(7)
+    table = torch.tensor([[0, 3], [-1, 1 << 20]], dtype=torch.int32, device="cuda")
+    pos = torch.tensor([16, 32, 1 << 30, -1, 0, 16, 0, 5], dtype=torch.int32, device="cuda")
+    slots = torch.tensor([0, 0, 1, 1, 1, 1, 2, 0], dtype=torch.int32, device="cuda")
+    qkv = torch.randn((8, (q_heads + 2 * kv_heads) * dim), generator=gen(23), device="cuda").to(torch.bfloat16)
+    q_out = torch.empty((8, q_heads * dim), dtype=torch.bfloat16, device="cuda")
+    ops.qk_norm_rope_store_fp8(qkv, None, None, 1.0, None, 0, pos, slots, table, planes, page, q_out, q_heads, kv_heads, dim, ops.QK_STORE | ops.QK_QOUT)
+    assert torch.equal(q_out, qkv[:, :q_heads * dim])
+    held = planes[2].view(torch.float32)[0, :, 5].clone()
+    assert (held > 0).all() and (held < 1).all()
+    for plane in planes:
+        plane[0, :, 5] = 7                                        # the one row with a place
+        assert (plane == 7).all()

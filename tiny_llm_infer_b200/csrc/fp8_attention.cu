@@ -10,7 +10,7 @@
 // come from HBM once per group: 2 hd + 8 bytes, half of the bfloat16 cache's.  What bounds it is their way from HBM.  The four warps take
 // units of 32 keys in turn: cp.async brings a unit's keys, values and scales into the warp's own ring of two while the unit before is
 // worked on; keys that do not count (behind the row's position, before its window, without a page) arrive as zeros, so that what a page
-// held before meets no sum.
+// held before meets no sum; a row left without keys becomes zeros.
 //
 // Products run on mma.sync m16n8k16 with float16 operands, which hold every e4m3 value exactly; keys and values are the left operands
 // (16 keys, or 16 dims, by 16) and eight query heads the right one, so a group of up to eight heads wastes nothing.  Queries are brought to
@@ -50,6 +50,9 @@ struct A8Unit {
 struct A8Cache {
     const uint8_t *k, *v, *scales;
     long long stride;             // bytes from one page to the next
+    int pages;
+    // a page of the table, or -1 where it names none: no other memory is read for it
+    __device__ __forceinline__ int held(int page) const { return (unsigned)page < (unsigned)pages ? page : -1; }
 };
 
 // Four bytes of two keys, interleaved: the first two dims' pairs, and the last two's.
@@ -144,18 +147,20 @@ __device__ __forceinline__ void attend_run(unsigned char* smem, const A8Row& row
     const uint8_t* const k0 = cache.k + lane * 16;
     const uint8_t* const v0 = cache.v + lane * 16;
     const int key_dst = Unit::key_at(lane / (HD / 16), lane % (HD / 16));
+    uint32_t gaps = 0;                                             // bit s: the unit in stage s has keys that no page holds
     // its two pages are looked up a unit ahead, so that no copy waits for the table
     int page[2];
     auto look_up = [&]() {
         const bool there = f_unit < unit_end, wraps = in_page + 16 >= page_size;
-        page[0] = there ? table[page_at] : -1;                                     // its first key is at or before pos
-        page[1] = there && key0 + 16 <= pos ? (wraps ? table[page_at + 1] : page[0]) : -1;
+        page[0] = there ? cache.held(table[page_at]) : -1;                         // its first key is at or before pos
+        page[1] = there && key0 + 16 <= pos ? (wraps ? cache.held(table[page_at + 1]) : page[0]) : -1;
     };
     look_up();
     auto fetch = [&]() {
         if (f_unit < unit_end) {
             const bool wraps = in_page + 16 >= page_size;
             const uint32_t dst = smem_u32(ring + (size_t)f_stage * Unit::kBytes);
+            gaps = (gaps & ~(1u << f_stage)) | (uint32_t)((page[0] | page[1]) < 0) << f_stage;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int first = key0 + 16 * h;
@@ -276,7 +281,7 @@ __device__ __forceinline__ void attend_run(unsigned char* smem, const A8Row& row
                 }
             }
         const int first = base + unit * kA8Unit + gr;
-        const bool whole = base + unit * kA8Unit >= lo && base + unit * kA8Unit + kA8Unit - 1 <= pos;
+        const bool whole = base + unit * kA8Unit >= lo && base + unit * kA8Unit + kA8Unit - 1 <= pos && !(gaps >> stage & 1);
         float lv[2][2];                                            // log2 of the values' scales, keys 16 h + gr + 8 e
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -295,7 +300,7 @@ __device__ __forceinline__ void attend_run(unsigned char* smem, const A8Row& row
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int j = first + 16 * h + 8 * e;
-                    if (j >= lo && j <= pos) continue;
+                    if (j >= lo && j <= pos && lv[h][e] != -INFINITY) continue;        // a scale of zero: copied from no page
                     lv[h][e] = -INFINITY;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
@@ -416,16 +421,24 @@ __device__ __forceinline__ void run_sums(const unsigned char* smem, int row, int
 __device__ __forceinline__ int first_key(int pos, int window) { return window > 0 && pos - window + 1 > 0 ? pos - window + 1 : 0; }
 __device__ __forceinline__ int units_of(int pos, int window) { return (pos - first_key(pos, window) / 16 * 16) / kA8Unit + 1; }
 
-// A row's position, held within what its row of the block table has room for: a caller's mistake reads no other memory.
-__device__ __forceinline__ int position_of(const int* positions, int r, int room) { return min(positions[r], room - 1); }
-
 struct A8Step {
     const bf16* q;
     A8Cache cache;
     const int *positions, *token_slot, *rows, *block_table;
-    int n_rows, max_pages, page_size, q_heads, kv_heads, window, room;      // room: max_pages * page_size
+    int n_rows, slots, max_pages, page_size, q_heads, kv_heads, window, room;       // room: max_pages * page_size
     float scale_log2e;
 };
+// A caller's mistake reads no other memory: a row's position is held within what its row of the block table has room for, and a slot without
+// a row of the table, or a position before the first key, is no request.
+__device__ __forceinline__ int position_of(const A8Step& st, int r) { return min(st.positions[r], st.room - 1); }
+__device__ __forceinline__ int slot_of(const A8Step& st, int r) {
+    const int slot = st.token_slot[r];
+    return slot < st.slots && st.positions[r] >= 0 ? slot : -1;
+}
+// Sums in float32 brought to an output; nothing where no key counted.
+__device__ __forceinline__ bf16 weighed(float acc, float dn, float total) {
+    return __float2bfloat16_rn(total == 0.0f ? 0.0f : acc * (dn == -INFINITY ? 0.0f : exp2f(dn - kA8Lift)) / total);
+}
 template <int HD>
 __device__ __forceinline__ A8Row row_at(const A8Step& st, int r, int slot, int g) {
     A8Row x;
@@ -435,7 +448,7 @@ __device__ __forceinline__ A8Row row_at(const A8Step& st, int r, int slot, int g
     x.table = st.block_table + (size_t)slot * st.max_pages;
     x.page_size = st.page_size;
     x.kv_heads = st.kv_heads;
-    x.pos = position_of(st.positions, r, st.room);
+    x.pos = position_of(st, r);
     x.lo = first_key(x.pos, st.window);
     x.base = x.lo / 16 * 16;
     x.scale_log2e = st.scale_log2e;
@@ -449,7 +462,7 @@ __global__ void __launch_bounds__(kA8Warps * 32, NT == 1 ? 3 : 2) attention_fp8_
     TLLM_PDL_ENTER();
     const int g = blockIdx.x, ridx = blockIdx.y;
     const int r = st.rows ? st.rows[ridx] : ridx, group = st.q_heads / st.kv_heads;
-    const int slot = st.token_slot[r];
+    const int slot = slot_of(st, r);
     bf16* dst = out + ((size_t)r * st.q_heads + (size_t)g * group) * HD;
     if (slot < 0) {
         for (int i = threadIdx.x; i < group * HD; i += blockDim.x) dst[i] = __float2bfloat16_rn(0.0f);
@@ -460,7 +473,7 @@ __global__ void __launch_bounds__(kA8Warps * 32, NT == 1 ? 3 : 2) attention_fp8_
     for (int i = threadIdx.x; i < group * HD; i += blockDim.x) {
         float acc, total, mm, dn;
         run_sums<HD, NT>(smem, i / HD, i % HD, acc, total, mm, dn);
-        dst[i] = __float2bfloat16_rn(acc * (dn == -INFINITY ? 0.0f : exp2f(dn - kA8Lift)) / total);
+        dst[i] = weighed(acc, dn, total);
     }
 }
 
@@ -472,8 +485,8 @@ __global__ void __launch_bounds__(kA8Warps * 32, NT == 1 ? 3 : 2) attention_fp8_
 // A (row, head) that one block has whole is written; pieces go to scratch.  Place of a chunk: its block; of the piece of (row, head) i in share b:
 // i + b (no two pieces have the same, as every next piece is of the next pair, the next share or both).  Chunks and shares are whole rounds of the
 // four warps.  plan: the chunks (units) of a head before each row, then 0 (the length of a share): the first block leaves it for the kernel
-// that adds the pieces.  (A grid of equal runs per row, whose lengths differ: 64 rows of 1000 to 4096 keys 86 us however finely cut, in shares 78;
-// shares alone, 8 rows of 500 to 2000 keys 21 us, as some blocks work on two pieces one after the other, in chunks 15.)
+// that adds the pieces.  (A grid of equal runs per row, whose lengths differ: 64 rows of 1000 to 4096 keys 86 us however finely cut, in shares 73;
+// shares alone, 8 rows of 500 to 2000 keys 21 us, as some blocks work on two pieces one after the other, in chunks 16.)
 constexpr int kA8MaxRows = 512, kA8MaxShares = 512;
 template <int HD, int NT>
 __global__ void __launch_bounds__(kA8Warps * 32, NT == 1 ? 3 : 2)
@@ -485,7 +498,7 @@ attention_fp8_share_kernel(const A8Step st, int* __restrict__ plan, float* __res
     int some = 0, rows_here = 0;
     for (int ridx = threadIdx.x; ridx < st.n_rows; ridx += kA8Warps * 32) {
         const int r = st.rows ? st.rows[ridx] : ridx;
-        const int pos = position_of(st.positions, r, st.room), slot = st.token_slot[r];
+        const int pos = position_of(st, r), slot = slot_of(st, r);
         const int n = slot >= 0 ? units_of(pos, st.window) : 0;
         units[ridx] = n;                                           // read back by this thread alone
         some += n;
@@ -568,7 +581,7 @@ attention_fp8_share_kernel(const A8Step st, int* __restrict__ plan, float* __res
             float acc, sum, mm, dn;
             run_sums<HD, NT>(smem, row, d, acc, sum, mm, dn);
             if (whole) {
-                out[((size_t)r * st.q_heads + (size_t)g * group) * HD + i] = __float2bfloat16_rn(acc * (dn == -INFINITY ? 0.0f : exp2f(dn - kA8Lift)) / sum);
+                out[((size_t)r * st.q_heads + (size_t)g * group) * HD + i] = weighed(acc, dn, sum);
             } else {
                 part_o[(place + row) * HD + d] = acc;
                 if (d == 0) { part_m[(place + row) * 3] = mm; part_m[(place + row) * 3 + 1] = dn; part_m[(place + row) * 3 + 2] = sum; }
@@ -593,7 +606,7 @@ attention_fp8_join_kernel(const A8Step st, const int* plan, const float* part_o,
     __shared__ float sums[WIDE ? kA8JoinWarps : 1][HD];
     TLLM_PDL_ENTER();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5, ridx = blockIdx.y;       // WIDE: kA8JoinWarps warps
-    const int r = st.rows ? st.rows[ridx] : ridx, group = st.q_heads / st.kv_heads, slot = st.token_slot[r];
+    const int r = st.rows ? st.rows[ridx] : ridx, group = st.q_heads / st.kv_heads, slot = slot_of(st, r);
     const int before = plan[ridx], n = plan[ridx + 1] - before, each = plan[st.n_rows + 1];
     const int g = WIDE ? blockIdx.x / group : blockIdx.x;
     const int start = before * st.kv_heads + g * n, b0 = each == 0 ? start : start / each;
@@ -672,9 +685,8 @@ attention_fp8_join_kernel(const A8Step st, const int* plan, const float* part_o,
 #pragma unroll
                 for (int e = 0; e < kDims; ++e) acc[e] += sums[i][lane * kDims + e];
         }
-        const float up = dn == -INFINITY ? 0.0f : exp2f(dn - kA8Lift);
 #pragma unroll
-        for (int e = 0; e < kDims; ++e) dst[e] = __float2bfloat16_rn(acc[e] * up / total);
+        for (int e = 0; e < kDims; ++e) dst[e] = weighed(acc[e], dn, total);
         if (WIDE) return;
     }
 }
@@ -731,7 +743,7 @@ __global__ void __launch_bounds__(256) attention_fp8_unpack_kernel(const A8Cache
     for (int s = 0; s < seg; ++s)
         if (seg_info[4 * s + 2] > 1 && seg_info[4 * s] >= 0)
             to += (seg_info[4 * s + 3] + seg_info[4 * s + 2] - 1) / page_size - first_page(seg_info[4 * s + 3]) + 1;
-    const int page = to < capacity ? block_table[(size_t)slot * max_pages + i] : -1;
+    const int page = to < capacity ? cache.held(block_table[(size_t)slot * max_pages + i]) : -1;
     if (threadIdx.x == 0) table[(size_t)slot * max_pages + i] = page < 0 ? -1 : to;
     if (page < 0) return;
     const size_t at = (size_t)page * cache.stride, plane = (size_t)kv_heads * page_size;
@@ -762,7 +774,8 @@ __global__ void __launch_bounds__(256) attention_fp8_unpack_kernel(const A8Cache
 
 using namespace tllm;
 
-static int check_a8(const char* what, const void* k, const void* v, const void* scales, long long page_bytes, int page_size, int kv_heads, int head_dim) {
+static int check_a8(const char* what, const void* k, const void* v, const void* scales, long long page_bytes, int pages, int page_size, int kv_heads, int head_dim) {
+    TLLM_REQUIRE(pages > 0, "%s: %d pages", what, pages);
     TLLM_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim %d is not 64 or 128", what, head_dim);
     TLLM_REQUIRE(kv_heads > 0 && kv_heads <= 65535, "%s: %d key/value heads", what, kv_heads);
     TLLM_REQUIRE(page_size > 0 && page_size % 16 == 0, "%s: page size %d is no multiple of 16", what, page_size);
@@ -772,15 +785,15 @@ static int check_a8(const char* what, const void* k, const void* v, const void* 
     return 0;
 }
 
-// q, out [rows, q_heads * head_dim] bfloat16; planes of pages `page_bytes` apart: k, v [kv_heads][page_size][head_dim] e4m3, scales
+// q, out [rows, q_heads * head_dim] bfloat16; block_table [slots][max_pages]; planes of `pages` pages `page_bytes` apart: k, v [kv_heads][page_size][head_dim] e4m3, scales
 // [kv_heads][page_size][2] float32.  rows: indices of the one-token rows, null for 0 .. n_rows - 1.  blocks: 0 for a block of threads per (row,
 // key/value head), else how many share all rows' keys (at most 512 rows and 512 blocks); then scratch, 16-byte aligned: float [(n_rows * kv_heads + blocks) *
 // (q_heads / kv_heads) * (head_dim + 3)], int [n_rows + 2].
 extern "C" int tllm_attention_fp8_decode(const void* q, const void* k, const void* v, const void* scales, long long page_bytes,
-                                         const int* positions, const int* token_slot, const int* rows, int n_rows, const int* block_table,
-                                         int max_pages, int page_size, int q_heads, int kv_heads, int head_dim, int window, float scale,
+                                         int pages, const int* positions, const int* token_slot, const int* rows, int n_rows,
+                                         const int* block_table, int slots, int max_pages, int page_size, int q_heads, int kv_heads, int head_dim, int window, float scale,
                                          int blocks, float* scratch, void* out, cudaStream_t stream) {
-    if (check_a8("attention_fp8_decode", k, v, scales, page_bytes, page_size, kv_heads, head_dim) != 0) return -1;
+    if (check_a8("attention_fp8_decode", k, v, scales, page_bytes, pages, page_size, kv_heads, head_dim) != 0) return -1;
     TLLM_REQUIRE(q_heads > 0 && q_heads % kv_heads == 0 && q_heads / kv_heads <= 16,
                  "attention_fp8_decode: %d query heads over %d key/value heads (at most 16 per group)", q_heads, kv_heads);
     TLLM_REQUIRE(n_rows >= 0 && n_rows <= 65535 && q_heads <= 65535 && max_pages > 0 && window >= 0 && (long long)max_pages * page_size <= 0x7fffffff,
@@ -792,8 +805,8 @@ extern "C" int tllm_attention_fp8_decode(const void* q, const void* k, const voi
     TLLM_REQUIRE(q && out && positions && token_slot && block_table && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(scratch)) & 15u) == 0,
                  "attention_fp8_decode: missing or unaligned operands");
     if (n_rows == 0) return 0;
-    const A8Step st{(const bf16*)q, A8Cache{(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)scales, page_bytes}, positions, token_slot, rows,
-                    block_table, n_rows, max_pages, page_size, q_heads, kv_heads, window, max_pages * page_size, scale * 1.4426950408889634f};
+    const A8Step st{(const bf16*)q, A8Cache{(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)scales, page_bytes, pages}, positions, token_slot, rows,
+                    block_table, n_rows, slots, max_pages, page_size, q_heads, kv_heads, window, max_pages * page_size, scale * 1.4426950408889634f};
     const int group = q_heads / kv_heads;
     const size_t places = ((size_t)n_rows * kv_heads + blocks) * group;
     float *part_o = scratch, *part_m = scratch + places * head_dim;
@@ -808,16 +821,16 @@ extern "C" int tllm_attention_fp8_decode(const void* q, const void* k, const voi
 #undef ATTEND
 }
 
-// seg_info [segments][4] = slot, first row, tokens, position of the first.  `per`: pages of the portion that has most; pages bfloat16
+// `held`: pages of the cache.  seg_info [segments][4] = slot, first row, tokens, position of the first.  `per`: pages of the portion that has most; pages bfloat16
 // [capacity][2][kv_heads][page_size][head_dim], room for all portions' pages; table int32 like block_table.
-extern "C" int tllm_attention_fp8_unpack(const void* k, const void* v, const void* scales, long long page_bytes, const int* seg_info, int segments,
+extern "C" int tllm_attention_fp8_unpack(const void* k, const void* v, const void* scales, long long page_bytes, int held, const int* seg_info, int segments,
                                          const int* block_table, int max_pages, int page_size, int kv_heads, int head_dim, int window, int per,
                                          int capacity, void* pages, int* table, cudaStream_t stream) {
-    if (check_a8("attention_fp8_unpack", k, v, scales, page_bytes, page_size, kv_heads, head_dim) != 0) return -1;
+    if (check_a8("attention_fp8_unpack", k, v, scales, page_bytes, held, page_size, kv_heads, head_dim) != 0) return -1;
     TLLM_REQUIRE(segments > 0 && segments <= 65535 && per > 0 && per <= max_pages && capacity > 0, "attention_fp8_unpack: bad sizes");
     TLLM_REQUIRE(seg_info && block_table && pages && table && (reinterpret_cast<uintptr_t>(pages) & 15u) == 0, "attention_fp8_unpack: missing operands");
     TLLM_REQUIRE((long long)2 * kv_heads * page_size * (head_dim / 16) <= 0x7fffffff, "attention_fp8_unpack: too large");
-    const A8Cache cache{(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)scales, page_bytes};
+    const A8Cache cache{(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)scales, page_bytes, held};
     if (head_dim == 64)
         launch_pdl(kPdlOther, attention_fp8_unpack_kernel<64>, dim3(per, segments), dim3(256), 0, stream, cache, seg_info, block_table, max_pages,
                    page_size, kv_heads, window, capacity, (bf16*)pages, table);

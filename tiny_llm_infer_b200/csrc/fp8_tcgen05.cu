@@ -4,16 +4,19 @@
 //   y[t, n] = sum_b sx[t, b] sw[n / 128, b] P_b[t, n],   P_b = the float32 product of block b's 128 k's.
 //
 // The scales differ from block to block of K, so no accumulator can run over all of K: the tensor core makes P_b alone (four
-// MMAs of 128 x BN x 32) in tensor memory, and eight warps multiply it by its scales and add it to float32 sums in registers while the
-// next P_b is being made.  Per block and tile of 128 x 256 the MMAs take 512 cycles, the reads of tensor memory 256 and the
-// multiply-adds 256, side by side.
+// MMAs over 32 k's each) in tensor memory, and eight warps multiply it by its scales and add it to float32 sums in registers while the
+// next P_b is being made.
 //
-// Warps: 0 fetches (TMA, 128-byte swizzle: a row of 128 e4m3 is one swizzle row), 1 issues MMAs and owns the tensor memory, 2 to 9 sum.
-// A summing thread owns one row and half of the tile's columns, one block of 128 weight rows, so that a block's scale is one number per thread (two
-// for interleaved gate and up rows).  Persistent: one block of threads per SM walks over tiles, row tiles fastest; with few tiles K is
-// cut into shares whose float32 sums a second kernel adds in order.
+// Two kernels.  Pairs of SMs make tiles of 256 x 256 (below); they carry the large products and the gated one.  Where those tiles would
+// be too few, single SMs make tiles of 128 x 128, and with fewer still K is cut into shares whose float32 sums a third kernel adds in
+// order (2048 x 6144 x 4096: pairs 51 us, which is 2.0 PFLOP/s; 61 x 4096 x 4096 in 4 shares: 11 us with the rows' rounding and the join).
 //
-// GATED: w's rows are gate and up interleaved by eight, the tile's 256 rows make 128 outputs act(gate) * up, one scale block
+// Warps of the 128 x 128 kernel: 0 fetches (TMA, 128-byte swizzle: a row of 128 e4m3 is one swizzle row), 1 and 2 issue MMAs in turn, 3 to
+// 10 sum.  A summing thread owns one row and half of the tile's columns, within one block of 128 weight rows, so that a block's scale
+// is one number per thread (two for interleaved gate and up rows).  Persistent: one block of threads per SM walks over tiles, row
+// tiles fastest.  A block of K costs it 0.37 us, bound by the way wait - MMA - commit - read of tensor memory, not by the MMAs.
+//
+// GATED: w's rows are gate and up interleaved by eight, a pair's 256 columns make 128 outputs act(gate) * up, one scale block
 // of the next product's rows, so they leave as e4m3 with their scale.
 //
 // Waits are bounded as in gemm_tcgen05.cu.
@@ -341,10 +344,13 @@ fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
 
 // ---------------------------------------------------------------- pairs of SMs
 // Tiles of 256 x 256 by two SMs (cta_group::2): each holds 128 rows of x and half of the 256 weight rows, and the tensor cores of both
-// read both halves, so a block of K costs an SM 32 KB from L2 in place of 48 for the same MMAs.  One thread of the first SM issues for
-// both; sums of 128 x 256 stay with each SM, whose eight summing warps take two numbers per instruction (fma.f32x2) while the next
-// 32 columns are on their way from tensor memory.  Those warps hold 128 sums a thread: registers go to them from the warpgroup that
+// read both halves, so a block of K costs an SM 32 KB from L2 in place of 48 for the same MMAs.  Two warps of the first SM issue for
+// both; sums of 128 x 256 stay with each SM, whose eight summing warps read 64 columns at a time and take two numbers per
+// instruction (fma.f32x2).  Those warps hold 128 sums a thread: registers go to them from the warpgroup that
 // fetches and issues (384 threads of 168 at launch: 4 warps of 40 and 8 of 232).
+// A block of K takes 0.47 us, of which the MMAs are 0.27: tensor memory holds two blocks' products, so a block's way through wait, MMAs,
+// commit and read is what bounds it (the tensor pipe is active for 55% of the time).  A block's MMAs cut in halves of 128 columns, each
+// with a commit of its own, took 63 us where this takes 57 (2048 x 6144 x 4096 with the rows' rounding).
 constexpr int kPairThreads = 384, kPairStages = 6, kPairStage = 2 * 128 * kQK;
 constexpr int kPairFetchRegs = 40, kPairSumRegs = 232;
 

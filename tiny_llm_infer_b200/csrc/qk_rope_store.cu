@@ -153,6 +153,7 @@ template <> struct HeadVec8<float> {
 struct Fp8Planes {
     uint8_t *k, *v, *scales;
     long long stride;             // bytes from one page to the next, the same in all three
+    int pages, slots;             // of the cache and rows of the block table: what names others, or a position behind the table's room, is not stored
 };
 template <typename T, typename TG, int HD, bool TABLE, int ROUNDS, typename TC>
 __global__ void __launch_bounds__(256) qk_norm_rope_store_vec_kernel(
@@ -209,7 +210,14 @@ __global__ void __launch_bounds__(256) qk_norm_rope_store_vec_kernel(
         for (int i = 0; i < 8; ++i) { gq[i] = to_f32<TG>(q_gain[e0 + i]); gk[i] = to_f32<TG>(k_gain[e0 + i]); }
     }
     int page = -1;
-    if (flags & kFlagStore) page = block_table[(size_t)slot * max_pages + pos / page_size];
+    if constexpr (std::is_same<TC, Fp8Planes>::value) {
+        if ((flags & kFlagStore) && slot < cache.slots && (unsigned)pos < (unsigned)max_pages * (unsigned)page_size) {
+            page = block_table[(size_t)slot * max_pages + pos / page_size];
+            if (page >= cache.pages) page = -1;
+        }
+    } else if (flags & kFlagStore) {
+        page = block_table[(size_t)slot * max_pages + pos / page_size];
+    }
     if constexpr (!TABLE) __syncthreads();
     // pair (i, i + HALF): x'_i = x_i cos a - x_{i+HALF} sin a; x'_{i+HALF} = x_i sin a + x_{i+HALF} cos a,
     // for both halves x' = x cos a + partner * (-+ sin a): cosines and signed sines of this lane's elements
@@ -400,8 +408,8 @@ extern "C" int tllm_qk_norm_rope_store(
 // says, keys, values and queries 16-byte aligned, `page_bytes` a multiple of 16.
 extern "C" int tllm_qk_norm_rope_store_fp8(
     void* qkv, const void* q_gain, const void* k_gain, int gain_dtype, float eps, const float* inv_freq, int rotary_dim,
-    const int* positions, const int* token_slot, const int* block_table, int max_pages, void* k_plane, void* v_plane, void* scales,
-    long long page_bytes, int page_size, void* q_out, int tokens, int q_heads, int kv_heads, int head_dim, int flags,
+    const int* positions, const int* token_slot, const int* block_table, int slots, int max_pages, void* k_plane, void* v_plane, void* scales,
+    long long page_bytes, int pages, int page_size, void* q_out, int tokens, int q_heads, int kv_heads, int head_dim, int flags,
     const float* rope_table, cudaStream_t stream) {
     TLLM_REQUIRE(tokens >= 0 && q_heads > 0 && kv_heads > 0, "qk_norm_rope_store_fp8: bad sizes");
     TLLM_REQUIRE(head_dim == 64 || head_dim == 128, "qk_norm_rope_store_fp8: head_dim %d is not 64 or 128", head_dim);
@@ -416,7 +424,7 @@ extern "C" int tllm_qk_norm_rope_store_fp8(
     TLLM_REQUIRE(al(qkv) && al(k_plane) && al(v_plane) && al(scales) && al(q_out) && al(rope_table) && page_bytes % 16 == 0,
                  "qk_norm_rope_store_fp8: operands must be 16-byte aligned");
     if (tokens == 0) return 0;
-    const Fp8Planes cache{(uint8_t*)k_plane, (uint8_t*)v_plane, (uint8_t*)scales, page_bytes};
+    const Fp8Planes cache{(uint8_t*)k_plane, (uint8_t*)v_plane, (uint8_t*)scales, page_bytes, pages, slots};
     const int per_block = 8 * (32 / (head_dim / 8));
     const int vgroups = tokens <= 64 ? (q_heads + 2 * kv_heads + per_block - 1) / per_block : 1;
     const bool table = rope_table != nullptr && (flags & kFlagRope), deep = tokens > 64;        // see ROUNDS above

@@ -45,10 +45,10 @@ def declare(h) -> None:
         "tllm_fp8_gated": [vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, f32, vp, vp, vp],
         "tllm_add_rmsnorm_fp8": [vp, vp, i32, vp, i32, f32, vp, vp, i32, i32, vp],
         "tllm_fp8_weight": [vp, i32, vp, vp, i32, i32, i32, vp],
-        "tllm_qk_norm_rope_store_fp8": [vp, vp, vp, i32, f32, vp, i32, vp, vp, vp, i32, vp, vp, vp, i64, i32, vp, i32, i32, i32, i32, i32,
-                                        vp, vp],
-        "tllm_attention_fp8_decode": [vp, vp, vp, vp, i64, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, f32, i32, vp, vp, vp],
-        "tllm_attention_fp8_unpack": [vp, vp, vp, i64, vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp],
+        "tllm_qk_norm_rope_store_fp8": [vp, vp, vp, i32, f32, vp, i32, vp, vp, vp, i32, i32, vp, vp, vp, i64, i32, i32, vp, i32, i32, i32, i32,
+                                        i32, vp, vp],
+        "tllm_attention_fp8_decode": [vp, vp, vp, vp, i64, i32, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, f32, i32, vp, vp, vp],
+        "tllm_attention_fp8_unpack": [vp, vp, vp, i64, i32, vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp],
     }
     for name, args in sigs.items():
         fn = getattr(h, name)
@@ -365,7 +365,7 @@ def cache_takes(page_size: int, q_heads: int, kv_heads: int, head_dim: int) -> b
 
 
 def _planes(planes, page_size: int, kv_heads: int, head_dim: int):
-    """(keys, values, scales, bytes from page to page) of an 8-bit cache's planes, checked."""
+    """(keys, values, scales, bytes from page to page, pages) of an 8-bit cache's planes, checked."""
     if len(planes) != 3:
         _refuse(f"an 8-bit cache has planes of keys, values and scales, got {len(planes)}")
     k, v, s = planes
@@ -377,7 +377,7 @@ def _planes(planes, page_size: int, kv_heads: int, head_dim: int):
             _refuse("an 8-bit cache's planes are dense within a page and equally far apart")
         if plane.get_device() != current:
             _refuse(f"a tensor of {plane.device}, the current device is cuda:{current}")
-    return k.data_ptr(), v.data_ptr(), s.data_ptr(), apart
+    return k.data_ptr(), v.data_ptr(), s.data_ptr(), apart, pages
 
 
 def _int32(what: str, *tensors) -> None:
@@ -390,7 +390,7 @@ def qk_norm_rope_store_fp8(qkv: torch.Tensor, q_gain, k_gain, eps: float, inv_fr
                            token_slot: torch.Tensor, block_table, planes, page_size: int, q_out, q_heads: int, kv_heads: int, head_dim: int,
                            flags: int, table: Optional[torch.Tensor] = None) -> None:
     """``qk_norm_rope_store`` into an 8-bit cache: ``planes`` = (keys, values, scales), ``cache_planes``.  bfloat16 rows, head widths 64 and
-    128, the whole head rotated or nothing."""
+    128, the whole head rotated or nothing.  What belongs to no slot, position or page that the table and the cache have is not stored."""
     ops = _ops()
     _here(qkv, q_gain, k_gain, inv_freq, positions, token_slot, block_table, q_out, table)
     _int32("qk_norm_rope_store_fp8", positions, token_slot, block_table)
@@ -410,11 +410,11 @@ def qk_norm_rope_store_fp8(qkv: torch.Tensor, q_gain, k_gain, eps: float, inv_fr
         _refuse("qk_norm_rope_store_fp8: gains of one type")
     if q_out is not None and (q_out.dtype != torch.bfloat16 or tuple(q_out.shape) != (tokens, q_heads * head_dim)):
         _refuse(f"qk_norm_rope_store_fp8: queries go to bfloat16 [{tokens}, {q_heads * head_dim}], got {q_out.dtype} {tuple(q_out.shape)}")
-    k, v, s, stride = _planes(planes, page_size, kv_heads, head_dim) if planes is not None else (None, None, None, 0)
+    k, v, s, stride, held = _planes(planes, page_size, kv_heads, head_dim) if planes is not None else (None, None, None, 0, 0)
     ops._check(ops.lib().tllm_qk_norm_rope_store_fp8(
         ops._p(qkv), ops._p(q_gain), ops._p(k_gain), ops._dt(q_gain) if q_gain is not None else ops.F32, float(eps), ops._p(inv_freq), rotary_dim,
-        ops._p(positions), ops._p(token_slot), ops._p(block_table), block_table.shape[1] if block_table is not None else 0, k, v, s, stride, page_size,
-        ops._p(q_out), tokens, q_heads, kv_heads, head_dim, flags, ops._p(table), ops._stream()), "qk_norm_rope_store_fp8")
+        ops._p(positions), ops._p(token_slot), ops._p(block_table),
+        *(block_table.shape if block_table is not None else (0, 0)), k, v, s, stride, held, page_size, ops._p(q_out), tokens, q_heads, kv_heads, head_dim, flags, ops._p(table), ops._stream()), "qk_norm_rope_store_fp8")
 
 
 def _attention_operands(what, q, out, positions, token_slot, rows, n_rows, block_table, q_heads, kv_heads, head_dim) -> None:
@@ -450,11 +450,12 @@ def paged_attention_decode_fp8(q, planes, positions, token_slot, rows, n_rows, b
     """Attention of one-token rows (``rows``: their indices, None for the first ``n_rows``) over an 8-bit paged cache, ``planes`` =
     (keys, values, scales): positions max(0, pos - window + 1) .. pos of the row's own request.  All rows' keys are cut into as many equal
     shares as there are ``blocks`` of threads, and a second kernel adds the pieces of a row in their order (0: one block per (row, key/value head),
-    one kernel; None: by ``attention_blocks``).  Rows with a negative slot become zeros; rows of ``out`` that are not asked for
+    one kernel; None: by ``attention_blocks``).  Rows of no request (a negative slot, or none of the table's; a negative position) become zeros, and so
+    do rows without a key; what no page of the cache holds does not count, and a position behind the table's room is held within it.  Rows of ``out`` that are not asked for
     stay as they are.  ``max_context``: no row's position is at or behind it (it sizes the grid)."""
     ops = _ops()
     _attention_operands("paged_attention_decode_fp8", q, out, positions, token_slot, rows, n_rows, block_table, q_heads, kv_heads, head_dim)
-    k, v, s, stride = _planes(planes, page_size, kv_heads, head_dim)
+    k, v, s, stride, held = _planes(planes, page_size, kv_heads, head_dim)
     max_pages = block_table.shape[1]
     if blocks is None:
         reach = min(max_context, max_pages * page_size)
@@ -463,8 +464,8 @@ def paged_attention_decode_fp8(q, planes, positions, token_slot, rows, n_rows, b
     if blocks:
         scratch = q.new_empty((n_rows * kv_heads + blocks) * (q_heads // kv_heads) * (head_dim + 3) + n_rows + 2, dtype=torch.float32)
     ops._check(ops.lib().tllm_attention_fp8_decode(
-        q.data_ptr(), k, v, s, stride, positions.data_ptr(), token_slot.data_ptr(), None if rows is None else rows.data_ptr(), n_rows,
-        block_table.data_ptr(), max_pages, page_size, q_heads, kv_heads, head_dim, window or 0, scale, blocks,
+        q.data_ptr(), k, v, s, stride, held, positions.data_ptr(), token_slot.data_ptr(), None if rows is None else rows.data_ptr(), n_rows,
+        block_table.data_ptr(), block_table.shape[0], max_pages, page_size, q_heads, kv_heads, head_dim, window or 0, scale, blocks,
         None if scratch is None else scratch.data_ptr(), out.data_ptr(), ops._stream()), "paged_attention_decode_fp8", 2 if blocks else 1)
     return out
 
@@ -495,12 +496,12 @@ def paged_attention_fp8(q, planes, positions, token_slot, block_table, page_size
                                    window, scale, out, ctx.max_context)
     if ctx.n_tiles:
         _attention_operands("paged_attention_fp8", q, out, positions, token_slot, None, tokens, block_table, q_heads, kv_heads, head_dim)
-        k, v, s, stride = _planes(planes, page_size, kv_heads, head_dim)
+        k, v, s, stride, held = _planes(planes, page_size, kv_heads, head_dim)
         segments, most = ctx.seg_info.shape[0], min(-(-ctx.max_context // page_size), block_table.shape[1])
         per, capacity = portion_pages(ctx, page_size, window, most, torch.cuda.is_current_stream_capturing())
         pages = torch.empty((capacity, 2, kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=q.device)
         table = torch.empty_like(block_table)
-        ops._check(ops.lib().tllm_attention_fp8_unpack(k, v, s, stride, ops._p(ctx.seg_info), segments, ops._p(block_table), block_table.shape[1], page_size,
+        ops._check(ops.lib().tllm_attention_fp8_unpack(k, v, s, stride, held, ops._p(ctx.seg_info), segments, ops._p(block_table), block_table.shape[1], page_size,
                                                        kv_heads, head_dim, int(window or 0), per, capacity, ops._p(pages), ops._p(table), ops._stream()),
                    "attention_fp8_unpack")
         ops._attention_tiles(q, pages, table, page_size, q_heads, kv_heads, head_dim, window, scale, out, ctx)
