@@ -132,3 +132,12 @@ def test_few_keys_have_a_block_of_their_own_and_many_are_shared():
     assert blocks(1, 8, 4, 64, 148) == blocks(16, 8, 2, 600, 148) == blocks(24, 8, 2, 1000, 148) == blocks(0, 8, 4, 9999, 148) == 0
     assert blocks(1, 8, 4, 1000, 148) == blocks(64, 8, 4, 4096, 148) == 444 and blocks(2, 1, 16, 100000, 148) == 296
     assert blocks(513, 8, 4, 100000, 148) == 0
+
+
+def test_a_weight_keeps_its_tensors():
+    """Its products know the tensors by their place: others make another weight."""
+    weight = ops.Fp8Weight(torch.zeros((16, 32), dtype=torch.float8_e4m3fn), torch.ones((1, 1)))
+    assert weight.q.shape == weight.shape and weight.scales.shape == (1, 1) and weight.dtype == torch.float8_e4m3fn
+    for name in ("q", "scales"):
+        with pytest.raises(AttributeError):
+            setattr(weight, name, getattr(weight, name).clone())

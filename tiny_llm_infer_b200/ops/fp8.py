@@ -82,7 +82,7 @@ class Fp8Weight:
     """A weight [N, K] as e4m3 values ``q`` and float32 ``scales`` [ceil(N / 128), ceil(K / 128)].  ``gated``: the rows are N / 2 gate
     and N / 2 up rows interleaved by eight (``ops.interleave_gate_up``), and the scales [2 ceil(N / 2 / 128), ceil(K / 128)] are those
     of 128 gate rows, of the up rows that belong to them, and so on.  K is a multiple of 16."""
-    __slots__ = ("q", "scales", "gated", "shape", "pointers", "index")
+    __slots__ = ("_q", "_scales", "gated", "shape", "device", "pointers", "index")
 
     def __init__(self, q: torch.Tensor, scales: torch.Tensor, gated: bool = False):
         if q.dtype != E4M3 or q.dim() != 2 or scales.dtype != torch.float32:
@@ -97,17 +97,22 @@ class Fp8Weight:
             _refuse(f"an 8-bit weight of {n} x {k} has scales {list(want)}, got {list(scales.shape)}")
         if q.device != scales.device or not q.is_contiguous() or not scales.is_contiguous() or q.data_ptr() % 16:
             _refuse("an 8-bit weight and its scales are contiguous on one device, the weight 16-byte aligned")
-        self.q, self.scales, self.gated = q, scales, bool(gated)
+        self._q, self._scales, self.gated = q, scales, bool(gated)
         # what every product asks for: the weight keeps its tensors, so their addresses are its own
-        self.shape, self.pointers, self.index = q.shape, (q.data_ptr(), scales.data_ptr()), q.get_device()
+        self.shape, self.device, self.index = q.shape, q.device, q.get_device()
+        self.pointers = (q.data_ptr(), scales.data_ptr())
+
+    @property
+    def q(self) -> torch.Tensor:
+        return self._q
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales
 
     @property
     def dtype(self):
-        return self.q.dtype
-
-    @property
-    def device(self):
-        return self.q.device
+        return E4M3
 
     def values(self) -> torch.Tensor:
         """The float32 numbers that the weight stands for (for tests and comparisons)."""
@@ -311,7 +316,7 @@ def linear_fp8(x, weight: Fp8Weight, out_dtype: Optional[torch.dtype] = None) ->
     code = ops._DT.get(want)
     if code is None:
         _refuse(f"unsupported dtype {want}")
-    n, device = weight.shape[0], weight.q.device
+    n, device = weight.shape[0], weight.device
     y = torch.empty((rows, n), dtype=want, device=device)
     if rows == 0:
         return y
@@ -332,7 +337,7 @@ def linear_swiglu_fp8(x, weight: Fp8Weight, act: str = "silu", consts=None) -> F
     rows, k, kind, values, scales = _rows_and_weight(x, weight)
     if not weight.gated:
         _refuse("linear_swiglu takes a gated 8-bit weight (gate and up rows interleaved by eight)")
-    n, device = weight.shape[0], weight.q.device
+    n, device = weight.shape[0], weight.device
     inter = n // 2
     _columns(inter)
     limit, slope = ops._consts(act, consts)
