@@ -87,6 +87,16 @@ CASES = [  # q_heads, kv_heads, dim, page, window, positions
 @pytest.mark.parametrize("splits", [None, 1, 2, 7, 64])
 @pytest.mark.parametrize("q_heads,kv_heads,dim,page,window,positions", CASES)
 def test_one_token_rows(q_heads, kv_heads, dim, page, window, positions, splits):
+    one_token_rows(q_heads, kv_heads, dim, page, window, positions, blocks=splits)
+
+
+@pytest.mark.parametrize("cluster", [1, 2, 4, 8])
+@pytest.mark.parametrize("q_heads,kv_heads,dim,page,window,positions", CASES)
+def test_one_token_rows_by_clusters(q_heads, kv_heads, dim, page, window, positions, cluster):
+    one_token_rows(q_heads, kv_heads, dim, page, window, positions, cluster=cluster)
+
+
+def one_token_rows(q_heads, kv_heads, dim, page, window, positions, **how):
     """Rows in another order than their slots, one of no request between them, rows not asked for left alone; what pages hold behind
     a request's last token, and pages of nobody, is NaN."""
     from tiny_llm_infer_b200 import ops
@@ -105,14 +115,14 @@ def test_one_token_rows(q_heads, kv_heads, dim, page, window, positions, splits)
     q = (torch.randn((total, q_heads * dim), generator=g, device="cuda") * 3).to(torch.bfloat16)
     out = torch.full_like(q, 7.0)
     scale = 1 / math.sqrt(dim)
-    ops.paged_attention_decode_fp8(q, planes, pos, slots, rows, n + 1, table, page, q_heads, kv_heads, dim, window or None, scale, out, max(lengths), splits)
+    ops.paged_attention_decode_fp8(q, planes, pos, slots, rows, n + 1, table, page, q_heads, kv_heads, dim, window or None, scale, out, max(lengths), **how)
     assert (out[0] == 0).all() and (out[-1] == 7).all()
     for i in range(n):
         r = n - 1 - i
         want, off = exact_row(q[1 + i].double().view(q_heads, dim), *kept[r], positions[r], window, scale)
         assert ((out[1 + i].double() - want).abs() <= off).all()
     again = torch.full_like(q, 7.0)
-    ops.paged_attention_decode_fp8(q, planes, pos, slots, rows, n + 1, table, page, q_heads, kv_heads, dim, window or None, scale, again, max(lengths), splits)
+    ops.paged_attention_decode_fp8(q, planes, pos, slots, rows, n + 1, table, page, q_heads, kv_heads, dim, window or None, scale, again, max(lengths), **how)
     assert torch.equal(out, again)
 
 
@@ -388,7 +398,7 @@ def test_many_rows_of_a_step():
     planes = planes_of(pages, kv_heads, page, dim)
     table = tables(g, lengths, page, pages, 44)
     fill(g, planes, table, lengths, page, (0.3, 0.3))
-    for total, blocks in ((512, 444), (512, 1), (700, 0), (700, None), (129, 512)):
+    for total, blocks in ((512, 444), (512, 1), (700, 0), (700, None), (240, 0), (256, None), (129, 512)):
         slots = torch.tensor([-1 if i % 7 == 3 else (i * 11) % 40 for i in range(total)], dtype=torch.int32, device="cuda")
         pos = torch.tensor([lengths[(i * 11) % 40] - 1 for i in range(total)], dtype=torch.int32, device="cuda")
         q = torch.randn((total, q_heads * dim), generator=g, device="cuda").to(torch.bfloat16)
@@ -406,9 +416,9 @@ def test_many_rows_of_a_step():
         ops.paged_attention_decode_fp8(q, planes, pos, slots, None, 129, table, page, q_heads, kv_heads, dim, None, 0.125, out, 700, 513)
 
 
-@pytest.mark.parametrize("blocks", [0, 30])
+@pytest.mark.parametrize("how", [dict(blocks=0), dict(blocks=30), dict(cluster=4), dict(cluster=8)])
 @pytest.mark.parametrize("dim", [64, 128])
-def test_what_no_page_holds_does_not_count(dim, blocks):
+def test_what_no_page_holds_does_not_count(dim, how):
     """Entries of the table without a page, or with one the cache does not have: their keys are left out, in the middle, at either end and
     everywhere; slots and positions of no request give zeros."""
     from tiny_llm_infer_b200 import ops
@@ -428,7 +438,7 @@ def test_what_no_page_holds_does_not_count(dim, blocks):
     q = torch.randn((n + 1, q_heads * dim), generator=g, device="cuda").to(torch.bfloat16)
     pos, slots = torch.cat([pos, pos[:1]]), torch.cat([slots, slots[-1:] + 1])          # and a slot behind the table
     out = torch.empty_like(q)
-    ops.paged_attention_decode_fp8(q, planes, pos, slots, None, n + 1, tabs, page, q_heads, kv_heads, dim, None, 0.125, out, length, blocks)
+    ops.paged_attention_decode_fp8(q, planes, pos, slots, None, n + 1, tabs, page, q_heads, kv_heads, dim, None, 0.125, out, length, **how)
     for r in range(n + 1):
         left = [j for j in range(pos[r] + 1) if r < n - 1 and j // page not in gone[r]]
         if not left:

@@ -127,11 +127,18 @@ def test_pages_of_portions():
     assert fp8.portion_pages(ctx, 16, 20, 40, capturing=True) == (40, 120)
 
 
-def test_few_keys_have_a_block_of_their_own_and_many_are_shared():
-    blocks = fp8.attention_blocks
-    assert blocks(1, 8, 4, 64, 148) == blocks(16, 8, 2, 600, 148) == blocks(24, 8, 2, 1000, 148) == blocks(0, 8, 4, 9999, 148) == 0
-    assert blocks(1, 8, 4, 1000, 148) == blocks(64, 8, 4, 4096, 148) == 444 and blocks(2, 1, 16, 100000, 148) == 296
-    assert blocks(513, 8, 4, 100000, 148) == 0
+def test_how_one_token_attention_is_cut():
+    """A block each where that is soon over or there are rows enough, a cluster each for a few longer rows, shares for a few of the longest."""
+    cut = fp8.attention_cut
+    assert cut(1, 8, 4, 64, 148) == cut(16, 8, 2, 600, 148) == cut(24, 8, 2, 1000, 148) == cut(64, 8, 4, 4096, 148) == cut(0, 8, 4, 9999, 148) == (0, 1)
+    assert cut(1, 8, 4, 4095, 148) == cut(1, 8, 4, 1000, 148) == (0, 8) and cut(8, 8, 4, 2000, 148) == (0, 4)
+    assert cut(2, 8, 4, 131072, 148) == (444, 1) and cut(2, 1, 16, 100000, 148) == (296, 1)
+    assert cut(513, 8, 4, 100000, 148) == (0, 1)
+    for rows in (1, 3, 17, 100, 512, 700):
+        for reach in (1, 129, 5000, 200000):
+            blocks, cluster = cut(rows, 8, 4, reach, 148)
+            assert cluster in (1, 2, 4, 8) and blocks in (0, 444) and (cluster == 1 or (blocks == 0 and rows * 8 * cluster <= 2.6 * 148))
+            assert blocks == 0 or rows <= 512
 
 
 def test_a_weight_keeps_its_tensors():

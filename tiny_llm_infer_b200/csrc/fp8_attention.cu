@@ -32,7 +32,7 @@
 namespace tllm {
 
 constexpr int kA8Warps = 4, kA8Unit = 32;        // keys a warp takes at a time
-constexpr int kA8Stages = 2;                     // units of a warp's ring: one in use, one on its way (8.4 KB at width 128)
+constexpr int kA8Stages = 2;                     // units of a warp's ring: one in use, one on its way (8.4 KB at width 128); more of them gained nothing
 constexpr float kA8Lift = 15.0f;                 // weights are 2^15 at most
 
 // A unit in shared memory: keys, values, pairs of scales.
@@ -139,26 +139,29 @@ __device__ __forceinline__ void attend_run(unsigned char* smem, const A8Row& row
     int unit = unit0 + warp;
     unsigned char* ring = smem + (size_t)warp * kA8Stages * Unit::kBytes;
 
-    // ---- the next unit to fetch: its first key, that key's page (index in the table) and place in it, for both of its sixteens
+    // ---- the next unit to fetch: its first key and that key's place in its page
     int f_unit = unit, f_stage = 0, key0 = base + unit * kA8Unit;
-    int page_at = key0 / page_size, in_page = key0 - page_at * page_size;
+    int in_page = key0 % page_size;
     constexpr int kStep = kA8Warps * kA8Unit;
-    const int step_pages = kStep / page_size, step_rest = kStep - step_pages * page_size;
+    const int step_rest = kStep % page_size;
     const uint8_t* const k0 = cache.k + lane * 16;
     const uint8_t* const v0 = cache.v + lane * 16;
     const int key_dst = Unit::key_at(lane / (HD / 16), lane % (HD / 16));
     uint32_t gaps = 0;                                             // bit s: the unit in stage s has keys that no page holds
-    // its two pages are looked up a unit ahead, so that no copy waits for the table
-    int page[2];
-    auto look_up = [&]() {
-        const bool there = f_unit < unit_end, wraps = in_page + 16 >= page_size;
-        page[0] = there ? cache.held(table[page_at]) : -1;                         // its first key is at or before pos
-        page[1] = there && key0 + 16 <= pos ? (wraps ? cache.held(table[page_at + 1]) : page[0]) : -1;
+    // The pages of sixteen units at once, a lane each for a sixteen of keys, and of the sixteen units after them: no copy waits for the table.
+    // (Looked up unit by unit, a unit ahead, a unit took a warp 1.2 us where it takes 0.9.)
+    auto look_up = [&](int first) {
+        const int mine = first + (lane >> 1) * kA8Warps;
+        if (first >= unit_end || mine >= unit_end) return -1;
+        const int key = base + mine * kA8Unit + (lane & 1) * 16;
+        return key <= pos ? table[key / page_size] : -1;
     };
-    look_up();
+    constexpr int kBatch = 16 * kA8Warps;
+    int listed = look_up(unit), listed_next = look_up(unit + kBatch), f_at = 0;
     auto fetch = [&]() {
         if (f_unit < unit_end) {
             const bool wraps = in_page + 16 >= page_size;
+            const int page[2] = {cache.held(__shfl_sync(0xffffffffu, listed, f_at)), cache.held(__shfl_sync(0xffffffffu, listed, f_at + 1))};
             const uint32_t dst = smem_u32(ring + (size_t)f_stage * Unit::kBytes);
             gaps = (gaps & ~(1u << f_stage)) | (uint32_t)((page[0] | page[1]) < 0) << f_stage;
 #pragma unroll
@@ -187,11 +190,11 @@ __device__ __forceinline__ void attend_run(unsigned char* smem, const A8Row& row
             }
             f_unit += kA8Warps;
             key0 += kStep;
-            page_at += step_pages;
             in_page += step_rest;
-            if (in_page >= page_size) in_page -= page_size, ++page_at;
+            if (in_page >= page_size) in_page -= page_size;
             f_stage = f_stage + 1 == kA8Stages ? 0 : f_stage + 1;
-            look_up();
+            f_at += 2;
+            if (f_at == 32) f_at = 0, listed = listed_next, listed_next = look_up(f_unit + kBatch);
         }
         cp_async_commit();                                         // one group per call, empty past the end
     };
@@ -455,12 +458,34 @@ __device__ __forceinline__ A8Row row_at(const A8Step& st, int r, int slot, int g
     return x;
 }
 
-// Short contexts: a block of threads per (row, key/value head), the whole of it one run.
-template <int HD, int NT>
+// A block of threads per (row, key/value head), the whole of it one run.  No kernel that follows may start before this one ends (and the same for clusters
+// below): bfloat16 products that start early hold their places and fetch beside it (eight layers of Qwen3-8B widths, 8 rows of 4096 keys: 1.39 ms
+// a step where it takes 0.89; one row 1.00 and 0.73).  ORDERED, for more blocks than are resident at once: the rows with most
+// keys first, so that what starts late is short (64 rows of 800 to 4096 keys, 8 heads of
+// 128: 56 us where equal shares took 64; sizes all alike are the one case that shares do better, 117 and 98).
+constexpr int kA8MaxOrdered = 256;
+template <int HD, int NT, bool ORDERED>
 __global__ void __launch_bounds__(kA8Warps * 32, NT == 1 ? 3 : 2) attention_fp8_whole_kernel(const A8Step st, bf16* __restrict__ out) {
     extern __shared__ __align__(128) unsigned char smem[];
-    TLLM_PDL_ENTER();
-    const int g = blockIdx.x, ridx = blockIdx.y;
+    TLLM_PDL_WAIT();
+    const int g = blockIdx.x;
+    int ridx = blockIdx.y;
+    if constexpr (ORDERED) {
+        __shared__ int units[kA8MaxOrdered], mine;
+        for (int i = threadIdx.x; i < st.n_rows; i += kA8Warps * 32) {
+            const int r = st.rows ? st.rows[i] : i;
+            units[i] = slot_of(st, r) >= 0 ? units_of(position_of(st, r), st.window) : 0;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < st.n_rows; i += kA8Warps * 32) {
+            const int n = units[i];
+            int ahead = 0;                                         // rows before this one: no two have as many
+            for (int j = 0; j < st.n_rows; ++j) ahead += units[j] > n || (units[j] == n && j < i);
+            if (ahead == (int)blockIdx.y) mine = i;
+        }
+        __syncthreads();
+        ridx = mine;
+    }
     const int r = st.rows ? st.rows[ridx] : ridx, group = st.q_heads / st.kv_heads;
     const int slot = slot_of(st, r);
     bf16* dst = out + ((size_t)r * st.q_heads + (size_t)g * group) * HD;
@@ -475,6 +500,69 @@ __global__ void __launch_bounds__(kA8Warps * 32, NT == 1 ? 3 : 2) attention_fp8_
         run_sums<HD, NT>(smem, i / HD, i % HD, acc, total, mm, dn);
         dst[i] = weighed(acc, dn, total);
     }
+}
+
+// Longer ones of few rows: a cluster of `size` blocks per (row, key/value head), each with an equal run of its keys, whose sums are added in
+// the order of the keys through distributed shared memory.  One kernel, no scratch, and no plan to be made before the first key is fetched.
+// (One row of 4095 keys for 32 heads on 8: 10.7 us, in shares 13.2, a block per head 34; 8 rows of up to 4096: 17 to 18, 20 to 23 and 34.)
+constexpr int kA8MaxCluster = 8;
+__device__ __forceinline__ float peer_float(uint32_t address, int rank) {
+    float v;
+    asm volatile("{\n\t.reg .b32 a;\n\t"
+                 "mapa.shared::cluster.u32 a, %1, %2;\n\t"
+                 "ld.shared::cluster.f32 %0, [a];\n\t}\n"
+                 : "=f"(v)
+                 : "r"(address), "r"(rank)
+                 : "memory");
+    return v;
+}
+template <int HD, int NT>
+__global__ void __launch_bounds__(kA8Warps * 32, NT == 1 ? 3 : 2) attention_fp8_cluster_kernel(const A8Step st, int size, bf16* __restrict__ out) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    constexpr size_t kJoined = (size_t)kA8Warps * 8 * NT * (HD + 3) * sizeof(float), kSums = (size_t)8 * NT * (HD + 3) * sizeof(float);
+    static_assert(kJoined + kSums <= (size_t)kA8Warps * kA8Stages * A8Unit<HD>::kBytes, "a block's sums lie behind its warps'");
+    TLLM_PDL_WAIT();
+    const int g = blockIdx.x / size, rank = (int)cluster_rank(), ridx = blockIdx.y;
+    const int r = st.rows ? st.rows[ridx] : ridx, group = st.q_heads / st.kv_heads;
+    const int slot = slot_of(st, r);
+    bf16* dst = out + ((size_t)r * st.q_heads + (size_t)g * group) * HD;
+    if (slot < 0) {                                                // for all of the cluster
+        for (int i = rank * blockDim.x + threadIdx.x; i < group * HD; i += size * blockDim.x) dst[i] = __float2bfloat16_rn(0.0f);
+        return;
+    }
+    const A8Row x = row_at<HD>(st, r, slot, g);
+    const int units = units_of(x.pos, st.window), each = ((units + size - 1) / size + kA8Warps - 1) / kA8Warps * kA8Warps;
+    const int u0 = min((long long)rank * each, (long long)units), u1 = min(u0 + each, units);
+    attend_run<HD, NT>(smem, x, st.cache, u0, u1);
+    float* o = reinterpret_cast<float*>(smem + kJoined);           // [8 NT][HD], then [8 NT][3]: M, D, sum
+    float* m = o + 8 * NT * HD;
+    for (int i = threadIdx.x; i < group * HD; i += kA8Warps * 32) {
+        float acc, total, mm, dn;
+        run_sums<HD, NT>(smem, i / HD, i % HD, acc, total, mm, dn);
+        o[i] = acc;
+        if (i % HD == 0) {
+            float* to = m + i / HD * 3;
+            to[0] = mm; to[1] = dn; to[2] = total;
+        }
+    }
+    __syncwarp();
+    cluster_sync();
+    const uint32_t o_at = smem_u32(o), m_at = smem_u32(m);
+    for (int i = rank * (kA8Warps * 32) + threadIdx.x; i < group * HD; i += size * kA8Warps * 32) {
+        float runs[kA8MaxCluster * 3], sums[kA8MaxCluster];
+#pragma unroll
+        for (int s = 0; s < kA8MaxCluster; ++s) {
+            const bool there = s < size;
+            sums[s] = there ? peer_float(o_at + i * 4, s) : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 3; ++e) runs[3 * s + e] = there ? peer_float(m_at + (i / HD * 3 + e) * 4, s) : e == 2 ? 0.0f : -INFINITY;
+        }
+        float acc, total, mm, dn;
+        join_runs<kA8MaxCluster>(runs, 3, sums, 1, kA8MaxCluster, acc, total, mm, dn);
+        dst[i] = weighed(acc, dn, total);
+    }
+    __syncwarp();
+    cluster_sync();                                                // no block leaves while its sums are read
 }
 
 // Longer ones: the keys of all rows shared by all blocks of threads, whatever the rows' lengths, in one of two ways.
@@ -692,18 +780,40 @@ attention_fp8_join_kernel(const A8Step st, const int* plan, const float* part_o,
 }
 
 template <int HD, int NT>
-static int launch_attention_fp8(const A8Step& st, int blocks, int* plan, float* part_o, float* part_m, void* out, cudaStream_t stream) {
+static int launch_attention_fp8(const A8Step& st, int blocks, int cluster, int* plan, float* part_o, float* part_m, void* out, cudaStream_t stream) {
     constexpr size_t ring = (size_t)kA8Warps * kA8Stages * A8Unit<HD>::kBytes, joined = (size_t)kA8Warps * 8 * NT * (HD + 3) * sizeof(float);
     constexpr size_t smem = ring > joined ? ring : joined;
     static OncePerDevice configured;
     if (configured.first()) {
-        cudaError_t e = cudaFuncSetAttribute(attention_fp8_whole_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        cudaError_t e = cudaFuncSetAttribute(attention_fp8_whole_kernel<HD, NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_fp8_whole_kernel<HD, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_fp8_cluster_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_fp8_share_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) { set_error("attention_fp8_decode: %s", cudaGetErrorString(e)); return (int)e; }
         configured.done();
     }
+    if (cluster > 1) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(cluster * st.kv_heads, st.n_rows);
+        cfg.blockDim = dim3(kA8Warps * 32);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = cluster;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, attention_fp8_cluster_kernel<HD, NT>, st, cluster, (bf16*)out);
+        if (e != cudaSuccess) { set_error("attention_fp8_cluster: %s", cudaGetErrorString(e)); return (int)e; }
+        return finish_launch("attention_fp8_cluster");
+    }
     if (blocks == 0) {
-        launch_pdl(kPdlAttention, attention_fp8_whole_kernel<HD, NT>, dim3(st.kv_heads, st.n_rows), dim3(kA8Warps * 32), smem, stream, st, (bf16*)out);
+        int sms = sm_count_cached();
+        if (sms <= 0) sms = 148;
+        auto kernel = st.n_rows <= kA8MaxOrdered && (long long)st.n_rows * st.kv_heads > (NT == 1 ? 3 : 2) * sms ? attention_fp8_whole_kernel<HD, NT, true>
+                                                                                                           : attention_fp8_whole_kernel<HD, NT, false>;
+        launch_pdl(kPdlAttention, kernel, dim3(st.kv_heads, st.n_rows), dim3(kA8Warps * 32), smem, stream, st, (bf16*)out);
         return finish_launch("attention_fp8_whole");
     }
     launch_pdl(kPdlAttention, attention_fp8_share_kernel<HD, NT>, dim3(blocks), dim3(kA8Warps * 32), smem, stream, st, plan, part_o, part_m, (bf16*)out);
@@ -787,12 +897,12 @@ static int check_a8(const char* what, const void* k, const void* v, const void* 
 
 // q, out [rows, q_heads * head_dim] bfloat16; block_table [slots][max_pages]; planes of `pages` pages `page_bytes` apart: k, v [kv_heads][page_size][head_dim] e4m3, scales
 // [kv_heads][page_size][2] float32.  rows: indices of the one-token rows, null for 0 .. n_rows - 1.  blocks: 0 for a block of threads per (row,
-// key/value head), else how many share all rows' keys (at most 512 rows and 512 blocks); then scratch, 16-byte aligned: float [(n_rows * kv_heads + blocks) *
+// key/value head), or with `cluster` (2, 4, 8) a cluster of them; else how many share all rows' keys (at most 512 rows and 512 blocks); then scratch, 16-byte aligned: float [(n_rows * kv_heads + blocks) *
 // (q_heads / kv_heads) * (head_dim + 3)], int [n_rows + 2].
 extern "C" int tllm_attention_fp8_decode(const void* q, const void* k, const void* v, const void* scales, long long page_bytes,
                                          int pages, const int* positions, const int* token_slot, const int* rows, int n_rows,
                                          const int* block_table, int slots, int max_pages, int page_size, int q_heads, int kv_heads, int head_dim, int window, float scale,
-                                         int blocks, float* scratch, void* out, cudaStream_t stream) {
+                                         int blocks, int cluster, float* scratch, void* out, cudaStream_t stream) {
     if (check_a8("attention_fp8_decode", k, v, scales, page_bytes, pages, page_size, kv_heads, head_dim) != 0) return -1;
     TLLM_REQUIRE(q_heads > 0 && q_heads % kv_heads == 0 && q_heads / kv_heads <= 16,
                  "attention_fp8_decode: %d query heads over %d key/value heads (at most 16 per group)", q_heads, kv_heads);
@@ -800,6 +910,8 @@ extern "C" int tllm_attention_fp8_decode(const void* q, const void* k, const voi
                  "attention_fp8_decode: bad grid");
     TLLM_REQUIRE(blocks >= 0 && blocks <= kA8MaxShares && (blocks == 0 || (n_rows <= kA8MaxRows && scratch)),
                  "attention_fp8_decode: %d rows shared by %d blocks (at most 512 and 512, with scratch)", n_rows, blocks);
+    TLLM_REQUIRE(cluster == 1 || (blocks == 0 && (cluster == 2 || cluster == 4 || cluster == kA8MaxCluster)),
+                 "attention_fp8_decode: clusters of %d blocks (1, 2, 4 or 8, without shares)", cluster);
     TLLM_REQUIRE(blocks == 0 || (long long)n_rows * kv_heads * ((long long)max_pages * page_size / kA8Unit + 1) < 0x7fffffff - (1 << 13),
                  "attention_fp8_decode: too many keys for shares");
     TLLM_REQUIRE(q && out && positions && token_slot && block_table && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(scratch)) & 15u) == 0,
@@ -811,7 +923,7 @@ extern "C" int tllm_attention_fp8_decode(const void* q, const void* k, const voi
     const size_t places = ((size_t)n_rows * kv_heads + blocks) * group;
     float *part_o = scratch, *part_m = scratch + places * head_dim;
     int* plan = reinterpret_cast<int*>(part_m + places * 3);
-#define ATTEND(HD, NT) return launch_attention_fp8<HD, NT>(st, blocks, plan, part_o, part_m, out, stream)
+#define ATTEND(HD, NT) return launch_attention_fp8<HD, NT>(st, blocks, cluster, plan, part_o, part_m, out, stream)
     if (head_dim == 64) {
         if (group <= 8) ATTEND(64, 1);
         ATTEND(64, 2);

@@ -354,14 +354,6 @@ fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
 constexpr int kPairThreads = 384, kPairStages = 6, kPairStage = 2 * 128 * kQK;
 constexpr int kPairFetchRegs = 40, kPairSumRegs = 232;
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
 // The address of the first SM's copy of something in shared memory.
 __device__ __forceinline__ uint32_t in_first(const void* p) {
     uint32_t a;

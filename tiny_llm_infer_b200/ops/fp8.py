@@ -47,7 +47,7 @@ def declare(h) -> None:
         "tllm_fp8_weight": [vp, i32, vp, vp, i32, i32, i32, vp],
         "tllm_qk_norm_rope_store_fp8": [vp, vp, vp, i32, f32, vp, i32, vp, vp, vp, i32, i32, vp, vp, vp, i64, i32, i32, vp, i32, i32, i32, i32,
                                         i32, vp, vp],
-        "tllm_attention_fp8_decode": [vp, vp, vp, vp, i64, i32, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, f32, i32, vp, vp, vp],
+        "tllm_attention_fp8_decode": [vp, vp, vp, vp, i64, i32, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, f32, i32, i32, vp, vp, vp],
         "tllm_attention_fp8_unpack": [vp, vp, vp, i64, i32, vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp],
     }
     for name, args in sigs.items():
@@ -436,41 +436,51 @@ def _attention_operands(what, q, out, positions, token_slot, rows, n_rows, block
 SHARED_ROWS = 512        # rows that may share blocks
 
 
-def attention_blocks(rows: int, kv_heads: int, group: int, reach: int, sms: int) -> int:
-    """Blocks of threads that share all rows' keys in ``paged_attention_decode_fp8`` (as many as are resident at once), or 0 for one block
-    per (row, key/value head) and no second kernel: whichever should take less.  A block of its own takes 3.5 us and 1.2 for every 128 of the
-    ``reach`` keys a row may see, nearly twice that where the resident blocks share HBM; shares take 10 us and 2.4 for every 32 keys that a warp gets, rows being
-    0.7 of the reach on average.  (us, own block and shares, rows x heads, reach: 1 x 8, 1000 11.5 and 9.0; 1 x 8, 4095 36 and 11; 8 x 8, 2000 25
-    and 16; 8 x 8, 4096 45 and 22; 64 x 8, 4096 83 and 73; 16 x 8, 600 10.6 and 12.7; 24 x 8 of width 64, 1000 13.1 and 14.9.)"""
-    if rows > SHARED_ROWS or rows == 0:
-        return 0
-    resident, pairs = (3 if group <= 8 else 2) * sms, rows * kv_heads
-    own = 3.5 + 1.2 * reach / 128 * max(1.0, 1.9 * pairs / resident)
-    shared = 10 + 2.4 * max(1.0, 0.7 * pairs * reach / 32 / (4 * resident))
-    return resident if shared < own else 0
+@functools.lru_cache(maxsize=8192)
+def attention_cut(rows: int, kv_heads: int, group: int, reach: int, sms: int):
+    """(blocks that share all rows' keys, blocks of a cluster) for ``paged_attention_decode_fp8``: (0, 1) for one block per (row, key/value head),
+    (0, 2 to 8) for a cluster of them, (as many as are resident, 1) for shares and a second kernel that adds them; whichever should take least,
+    in us, for rows of at most ``reach`` keys, 0.65 of them on average.  A block of its own: 4.1, and 0.9 for every 128 keys, up to 1.4 times that where
+    SMs have several, or what HBM takes for all keys.  A cluster: 5.4, 1 for every 100 blocks, and 0.95 to 1.3 for every 128 keys of a block.  Shares: 12, and 2.4
+    for every 32 keys that a warp gets.  (Measured, us, own block, cluster, shares, rows x heads of 128, longest: 1 x 8, 1000 12.2, 6.7, 10.0; 1 x 8, 4095
+    34, 10.7, 13.2; 1 x 8, 16384 117, 21.4, 18.7; 8 x 8, 1000 12.9, 10.3, 14.7; 8 x 8, 4095 34, 16.7, 20.1; 16 x 8, 4095 34, 25.9, 27.4; 24 x 8, 4096 41, 34, 35;
+    37 x 8, 4096 43, 54, 49; 64 x 8, 4096 56, -, 64, all equally long 117 and 98; 128 x 8, 4096 123, -, 129.)"""
+    if rows == 0:
+        return 0, 1
+    pairs, mean = rows * kv_heads, 0.65 + 0.35 / rows
+    resident = (3 if group <= 8 else 2) * sms
+    best = (4.1 + max(0.9 * -(-reach // 128) * min(1.4, 1 + pairs / 1000), 2.93e-5 * pairs * reach), 0, 1)
+    for size in (2, 4, 8):
+        if pairs * size <= 2.6 * sms:
+            best = min(best, (5.4 + pairs * size / 100 + 0.95 * -(-reach // (128 * size)) * (1 + pairs * size / 1000), 0, size))
+    if rows <= SHARED_ROWS:
+        best = min(best, (12 + 2.4 * max(1.0, mean * pairs * reach / 32 / (4 * resident)), resident, 1))
+    return best[1:]
 
 
 def paged_attention_decode_fp8(q, planes, positions, token_slot, rows, n_rows, block_table, page_size, q_heads, kv_heads, head_dim, window, scale,
-                               out, max_context, blocks=None):
+                               out, max_context, blocks=None, cluster=None):
     """Attention of one-token rows (``rows``: their indices, None for the first ``n_rows``) over an 8-bit paged cache, ``planes`` =
-    (keys, values, scales): positions max(0, pos - window + 1) .. pos of the row's own request.  All rows' keys are cut into as many equal
-    shares as there are ``blocks`` of threads, and a second kernel adds the pieces of a row in their order (0: one block per (row, key/value head),
-    one kernel; None: by ``attention_blocks``).  Rows of no request (a negative slot, or none of the table's; a negative position) become zeros, and so
-    do rows without a key; what no page of the cache holds does not count, and a position behind the table's room is held within it.  Rows of ``out`` that are not asked for
-    stay as they are.  ``max_context``: no row's position is at or behind it (it sizes the grid)."""
+    (keys, values, scales): positions max(0, pos - window + 1) .. pos of the row's own request.  One block of threads takes a
+    (row, key/value head), with ``cluster`` = 2, 4 or 8 that many together; with ``blocks`` (at most 512, for at most 512 rows) so many
+    share all rows' keys, and a second kernel adds the pieces of a row in their order (neither given: ``attention_cut``).  Rows of no
+    request (a negative slot, or none of the table's; a negative position) become zeros, and so do rows without a key; what no page of
+    the cache holds does not count, and a position behind the table's room is held within it.  Rows of ``out`` that are not asked for
+    stay as they are.  ``max_context``: no row's position is at or behind it (what is taken goes by it)."""
     ops = _ops()
     _attention_operands("paged_attention_decode_fp8", q, out, positions, token_slot, rows, n_rows, block_table, q_heads, kv_heads, head_dim)
     k, v, s, stride, held = _planes(planes, page_size, kv_heads, head_dim)
     max_pages = block_table.shape[1]
-    if blocks is None:
+    if blocks is None and cluster is None:
         reach = min(max_context, max_pages * page_size)
-        blocks = attention_blocks(n_rows, kv_heads, q_heads // kv_heads, min(reach, window) if window else reach, ops.SM_COUNT)
+        blocks, cluster = attention_cut(n_rows, kv_heads, q_heads // kv_heads, min(reach, window) if window else reach, ops.SM_COUNT)
+    blocks, cluster = blocks or 0, cluster or 1
     scratch = None
     if blocks:
         scratch = q.new_empty((n_rows * kv_heads + blocks) * (q_heads // kv_heads) * (head_dim + 3) + n_rows + 2, dtype=torch.float32)
     ops._check(ops.lib().tllm_attention_fp8_decode(
         q.data_ptr(), k, v, s, stride, held, positions.data_ptr(), token_slot.data_ptr(), None if rows is None else rows.data_ptr(), n_rows,
-        block_table.data_ptr(), block_table.shape[0], max_pages, page_size, q_heads, kv_heads, head_dim, window or 0, scale, blocks,
+        block_table.data_ptr(), block_table.shape[0], max_pages, page_size, q_heads, kv_heads, head_dim, window or 0, scale, blocks, cluster,
         None if scratch is None else scratch.data_ptr(), out.data_ptr(), ops._stream()), "paged_attention_decode_fp8", 2 if blocks else 1)
     return out
 
