@@ -19,7 +19,8 @@
 // GATED: w's rows are gate and up interleaved by eight, a pair's 256 columns make 128 outputs act(gate) * up, one scale block
 // of the next product's rows, so they leave as e4m3 with their scale.
 //
-// Waits are bounded as in gemm_tcgen05.cu.
+// Waits are bounded as in gemm_tcgen05.cu.  The kernels start while the one ahead still runs (programmatic dependent launch): every role waits for
+// its end before its first bounded wait.
 #include <cuda.h>
 
 #include "fp8.cuh"
@@ -267,6 +268,7 @@ fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         }
     } else if (warp < 3) {
         // two warps issue in turn (see the pairs below)
+        TLLM_PDL_WAIT();                                        // or the limit of the first wait runs over the kernel ahead's work
         constexpr uint32_t idesc = instr_desc_e4m3(kQM, BN);
         const uint32_t issue = lane == 0;
         int it = 0;                                              // blocks of the tiles before
@@ -456,6 +458,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             }
         } else if ((warp == 1 || warp == 2) && rank == 0) {
             // two warps issue in turn, one for each half of tensor memory: a warp's waits, issue and commit take as long as a block's MMAs
+            TLLM_PDL_WAIT();                                    // or the limit of the first wait runs over the kernel ahead's work
             constexpr uint32_t idesc = instr_desc_e4m3(256, 256);
             const uint32_t issue = lane == 0, acc = tmem_base + (warp - 1) * 256;
             const int blocks = (total - pair + pairs - 1) / pairs * p.kb_all;       // of all of this pair's tiles
