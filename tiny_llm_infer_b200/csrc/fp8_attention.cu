@@ -22,7 +22,8 @@
 // The softmax is online in float32 with two maxima: M of s_j for the denominator, and D of (s_j - M) + log2 sv_j for the weights
 // 2^((s_j - M) + log2 sv_j - D + 15) of the values, which are rounded to float16: relative to the heaviest term they keep 11 bits down to
 // 2^-29, whatever the values' scales, and what is lost below is under 2^-40 of it per key.  (D is relative to M, so that a score of any size
-// leaves the scale's logarithm its bits.)  The denominator sums unrounded numbers.
+// leaves the scale's logarithm its bits.)  The denominator sums unrounded numbers.  A value whose scale is zero, or below float32's normal
+// numbers, adds nothing, and its key counts in the denominator; scales are not negative.
 //
 // With the heads as rows of a 16-row tile and 16 keys at a time a warp took 1.0 us a tile alone and 1.8 us beside eleven others (2.9 to
 // 3.9 TB/s): half of every product was wasted on missing rows, and the chain of scores, maxima and weights was walked twice as often.
@@ -147,7 +148,7 @@ __device__ __forceinline__ void attend_run(unsigned char* smem, const A8Row& row
     const uint8_t* const k0 = cache.k + lane * 16;
     const uint8_t* const v0 = cache.v + lane * 16;
     const int key_dst = Unit::key_at(lane / (HD / 16), lane % (HD / 16));
-    uint32_t gaps = 0;                                             // bit s: the unit in stage s has keys that no page holds
+    uint32_t gaps = 0;                                             // bit 2 s + h: keys 16 h .. 16 h + 15 of the unit in stage s are in no page
     // The pages of sixteen units at once, a lane each for a sixteen of keys, and of the sixteen units after them: no copy waits for the table.
     // (Looked up unit by unit, a unit ahead, a unit took a warp 1.2 us where it takes 0.9.)
     auto look_up = [&](int first) {
@@ -163,7 +164,7 @@ __device__ __forceinline__ void attend_run(unsigned char* smem, const A8Row& row
             const bool wraps = in_page + 16 >= page_size;
             const int page[2] = {cache.held(__shfl_sync(0xffffffffu, listed, f_at)), cache.held(__shfl_sync(0xffffffffu, listed, f_at + 1))};
             const uint32_t dst = smem_u32(ring + (size_t)f_stage * Unit::kBytes);
-            gaps = (gaps & ~(1u << f_stage)) | (uint32_t)((page[0] | page[1]) < 0) << f_stage;
+            gaps = (gaps & ~(3u << 2 * f_stage)) | ((uint32_t)page[0] >> 31 | (uint32_t)page[1] >> 31 << 1) << 2 * f_stage;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int first = key0 + 16 * h;
@@ -284,7 +285,8 @@ __device__ __forceinline__ void attend_run(unsigned char* smem, const A8Row& row
                 }
             }
         const int first = base + unit * kA8Unit + gr;
-        const bool whole = base + unit * kA8Unit >= lo && base + unit * kA8Unit + kA8Unit - 1 <= pos && !(gaps >> stage & 1);
+        const uint32_t missing = gaps >> 2 * stage & 3u;
+        const bool whole = base + unit * kA8Unit >= lo && base + unit * kA8Unit + kA8Unit - 1 <= pos && missing == 0;
         float lv[2][2];                                            // log2 of the values' scales, keys 16 h + gr + 8 e
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -303,7 +305,7 @@ __device__ __forceinline__ void attend_run(unsigned char* smem, const A8Row& row
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int j = first + 16 * h + 8 * e;
-                    if (j >= lo && j <= pos && lv[h][e] != -INFINITY) continue;        // a scale of zero: copied from no page
+                    if (j >= lo && j <= pos && !(missing >> h & 1)) continue;
                     lv[h][e] = -INFINITY;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)

@@ -465,7 +465,8 @@ def paged_attention_decode_fp8(q, planes, positions, token_slot, rows, n_rows, b
     (row, key/value head), with ``cluster`` = 2, 4 or 8 that many together; with ``blocks`` (at most 512, for at most 512 rows) so many
     share all rows' keys, and a second kernel adds the pieces of a row in their order (neither given: ``attention_cut``).  Rows of no
     request (a negative slot, or none of the table's; a negative position) become zeros, and so do rows without a key; what no page of
-    the cache holds does not count, and a position behind the table's room is held within it.  Rows of ``out`` that are not asked for
+    the cache holds does not count, and a position behind the table's room is held within it.  Scales are zero or more; a value whose scale
+    is zero counts with its key's weight.  Rows of ``out`` that are not asked for
     stay as they are.  ``max_context``: no row's position is at or behind it (what is taken goes by it)."""
     ops = _ops()
     _attention_operands("paged_attention_decode_fp8", q, out, positions, token_slot, rows, n_rows, block_table, q_heads, kv_heads, head_dim)
