@@ -1,0 +1,54 @@
+"""A model's 8-bit forms are taken whole or not at all; no GPU needed."""
+import pytest
+import torch
+
+from tiny_llm_infer_b200 import ops
+from tiny_llm_infer_b200.config.base import describe_model
+from tiny_llm_infer_b200.models.model import Model
+from tiny import TINIES
+
+
+def qwen():
+    model = Model(describe_model(TINIES["D"]["cfg"]), torch.bfloat16, "cpu")
+    model.loaded = True
+    assert len(model.blocks) > 1
+    return model
+
+
+def test_a_cache_that_one_mixer_cannot_keep_changes_none():
+    model = qwen()
+    model.blocks[-1].mixer.dtype = torch.float32
+    needs = model.cache_needs()
+    with pytest.raises(ValueError, match="8-bit cache"):
+        model.use_fp8_cache(16)
+    assert not model.fp8_cache and not any(m.cache_fp8 for b in model.blocks for m in b.mixers())
+    assert model.cache_needs() == needs
+
+
+@pytest.mark.parametrize("part", ["ffn", "mixer", "norm2"])
+def test_weights_that_one_part_cannot_keep_change_none(part, monkeypatch):
+    made = []
+    monkeypatch.setattr(ops, "quantize_weight_fp8", lambda w, gated=False: made.append(w))
+    model = qwen()
+    for block in model.blocks:                                  # 344 is no multiple of 16
+        block.ffn.inter = 352
+    last = model.blocks[-1]
+    if part == "norm2":
+        last.norm2.width = 32784                                # more than a row's kernel takes
+    else:
+        setattr(getattr(last, part), "hidden", 1032)
+    with pytest.raises(ValueError):
+        model.use_fp8_weights()
+    assert not made and not model.fp8_weights and not any(b.norm1.rows_fp8 or b.norm2.rows_fp8 for b in model.blocks)
+
+
+def test_a_model_of_parts_with_the_form_is_taken(monkeypatch):
+    made = []
+    monkeypatch.setattr(ops, "quantize_weight_fp8", lambda w, gated=False: made.append(gated))
+    model = qwen()
+    for block in model.blocks:
+        block.ffn.inter = 352
+    model.use_fp8_weights()
+    model.use_fp8_cache(16)
+    assert made == [False, False, True, False] * len(model.blocks) and model.fp8_weights and model.fp8_cache
+    assert all(b.norm1.rows_fp8 and b.norm2.rows_fp8 and b.mixer.cache_fp8 for b in model.blocks)

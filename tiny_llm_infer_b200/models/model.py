@@ -89,7 +89,7 @@ class Model:
     # ---- 8 bits
     def use_fp8_weights(self) -> None:
         """Keep the matrices of every block in 8 bits (once, after ``load``).  Embedding, norms and head stay as they are.  A block or
-        a part without that form is refused, and then nothing has changed its form that could still be run: build the model anew."""
+        a part without that form is refused before any has changed its own."""
         if not self.loaded:
             raise ValueError("weights are brought to 8 bits after they are loaded")
         if self.dtype != torch.bfloat16:
@@ -97,15 +97,19 @@ class Model:
         if self.fp8_weights:
             raise ValueError("the model's weights are in 8 bits already")
         for block in self.blocks:
+            block.check_fp8_weights()
+        for block in self.blocks:
             block.use_fp8_weights()
         self.fp8_weights = True
 
     def use_fp8_cache(self, page_size: int) -> None:
-        """Keep keys and values in 8 bits, from here on; cache managers for the model are then made with ``dtype=torch.uint8``."""
+        """Keep keys and values in 8 bits, from here on; cache managers for the model are then made with ``dtype=torch.uint8``.  A mixer
+        without that form is refused before any has changed its own."""
         mixers = [m for b in self.blocks for m in b.mixers()]
         for mixer in mixers:
             if not hasattr(mixer, "use_fp8_cache"):
                 raise ValueError(f"{type(mixer).__name__} has no 8-bit cache")
+            mixer.check_fp8_cache(page_size)
         for mixer in mixers:
             mixer.use_fp8_cache(page_size)
         self.fp8_cache = True

@@ -22,6 +22,7 @@ BLOCK = 128
 E4M3 = torch.float8_e4m3fn
 SMALLEST = 2.0 ** -100
 LARGEST = 448.0
+NORM_WIDTH = 32768       # columns that add_rmsnorm_fp8 takes
 
 
 _package = None

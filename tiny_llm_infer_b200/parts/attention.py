@@ -73,19 +73,27 @@ class GroupedQueryAttention:
             gd = torch.float32 if any(g.dtype == torch.float32 for g in gains) else gains[0].dtype
             self.q_gain, self.k_gain = (g.to(gd).contiguous() for g in gains)
 
-    def use_fp8_weights(self) -> None:
-        """The four projections as e4m3 values with scales."""
+    def check_fp8_weights(self) -> None:
+        """Refuses widths that 8-bit weights do not have."""
         if self.hidden % 16 or self.q_heads * self.head_dim % 16:
             raise ValueError(f"8-bit weights need widths that are multiples of 16: model {self.hidden}, heads {self.q_heads * self.head_dim}")
+
+    def use_fp8_weights(self) -> None:
+        """The four projections as e4m3 values with scales."""
+        self.check_fp8_weights()
         self.w_qkv, self.w_o = ops.quantize_weight_fp8(self.w_qkv), ops.quantize_weight_fp8(self.w_o)
 
-    def use_fp8_cache(self, page_size: int) -> None:
-        """Keys and values as e4m3 with a scale per token and head (``ops.fp8.cache_planes``)."""
+    def check_fp8_cache(self, page_size: int) -> None:
+        """Refuses what the 8-bit cache's kernels do not take."""
         fused = self.position is None or (hasattr(self.position, "fused_rotary") and (self.position.fused_rotary() or (None, None))[1] == self.head_dim)
         if self.dtype != torch.bfloat16 or not fused or not ops.fp8.cache_takes(page_size, self.q_heads, self.kv_heads, self.head_dim):
             raise ValueError(f"an 8-bit cache is for bfloat16 models, heads of 64 or 128 that turn whole, at most 16 query heads per key/value "
                              f"head and pages of a multiple of 16 tokens: {self.dtype}, {self.q_heads} and {self.kv_heads} heads of "
                              f"{self.head_dim}, pages of {page_size}")
+
+    def use_fp8_cache(self, page_size: int) -> None:
+        """Keys and values as e4m3 with a scale per token and head (``ops.fp8.cache_planes``)."""
+        self.check_fp8_cache(page_size)
         self.cache_fp8 = True
 
     # ---- what the cache manager has to provide

@@ -69,9 +69,13 @@ class Block:
         each a cache of its own)."""
         return [self.parts[role] for role, category in self.roles.items() if category == "mixer"]
 
+    def check_fp8_weights(self) -> None:
+        """Refuses, before anything has changed, what ``use_fp8_weights`` could not do."""
+        raise ValueError(f"blocks of kind {type(self).__name__} have no 8-bit weights")
+
     def use_fp8_weights(self) -> None:
         """Keep the sub-layers' matrices in 8 bits, and have the norms hand their rows on in 8 bits."""
-        raise ValueError(f"blocks of kind {type(self).__name__} have no 8-bit weights")
+        self.check_fp8_weights()
 
 
 @register("block", "prenorm")
@@ -85,13 +89,19 @@ class PreNormBlock(Block):
         x = self.norm2.forward(h, a)
         return self.ffn.forward(x, ctx)
 
-    def use_fp8_weights(self) -> None:
+    def check_fp8_weights(self) -> None:
         for role, part in self.parts.items():
-            if not hasattr(part, "use_fp8_weights" if self.roles[role] != "norm" else "rows_fp8"):
+            check = getattr(part, "check_fp8_rows" if self.roles[role] == "norm" else "check_fp8_weights", None)
+            if check is None:
                 raise ValueError(f"{type(part).__name__} has no 8-bit form")
+            check()
+
+    def use_fp8_weights(self) -> None:
+        super().use_fp8_weights()
         self.mixer.use_fp8_weights()
         self.ffn.use_fp8_weights()
-        self.norm1.rows_fp8 = self.norm2.rows_fp8 = True
+        self.norm1.use_fp8_rows()
+        self.norm2.use_fp8_rows()
 
 
 @register("block", "sandwich")

@@ -52,10 +52,14 @@ class SwiGLUFeedForward:
             self.w_gate_up = torch.cat([p.to(common) for p in parts], dim=0).contiguous()
         self.w_down = t[self.names[2]].contiguous()
 
-    def use_fp8_weights(self) -> None:
-        """Gate and up, and down, as e4m3 values with scales; the activation leaves its product as 8-bit rows."""
+    def check_fp8_weights(self) -> None:
+        """Refuses widths that 8-bit weights do not have."""
         if self.hidden % 16 or self.inter % 16:
             raise ValueError(f"8-bit weights need widths that are multiples of 16: model {self.hidden}, feed-forward {self.inter}")
+
+    def use_fp8_weights(self) -> None:
+        """Gate and up, and down, as e4m3 values with scales; the activation leaves its product as 8-bit rows."""
+        self.check_fp8_weights()
         self.w_gate_up = ops.quantize_weight_fp8(self.w_gate_up, gated=True)
         self.w_down = ops.quantize_weight_fp8(self.w_down)
 

@@ -68,6 +68,16 @@ class RMSNorm:
             gain = gain.to(torch.float32) + self.offset
         self.gain = gain.contiguous()
 
+    def check_fp8_rows(self) -> None:
+        """Refuses widths that ``ops.add_rmsnorm_fp8`` does not take."""
+        if self.width % 16 or self.width > ops.fp8.NORM_WIDTH:
+            raise ValueError(f"norms hand on 8-bit rows of a multiple of 16 up to {ops.fp8.NORM_WIDTH} columns, not {self.width}")
+
+    def use_fp8_rows(self) -> None:
+        """Hand rows on in 8 bits."""
+        self.check_fp8_rows()
+        self.rows_fp8 = True
+
     def wrap(self, delta: torch.Tensor) -> NormedDelta:
         """``delta`` with this norm still to be applied to it, by the norm that adds it to the stream."""
         return NormedDelta(delta, self.gain, self.eps)
