@@ -52,3 +52,14 @@ def test_a_model_of_parts_with_the_form_is_taken(monkeypatch):
     model.use_fp8_cache(16)
     assert made == [False, False, True, False] * len(model.blocks) and model.fp8_weights and model.fp8_cache
     assert all(b.norm1.rows_fp8 and b.norm2.rows_fp8 and b.mixer.cache_fp8 for b in model.blocks)
+
+
+def test_other_weights_are_not_loaded_over_8_bit_ones(monkeypatch):
+    """The norms already hand on 8-bit rows, which a bfloat16 matrix does not take."""
+    monkeypatch.setattr(ops, "quantize_weight_fp8", lambda w, gated=False: None)
+    model = qwen()
+    for block in model.blocks:
+        block.ffn.inter = 352
+    model.use_fp8_weights()
+    with pytest.raises(ValueError, match="8 bits"):
+        model.load({})

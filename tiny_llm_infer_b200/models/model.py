@@ -79,6 +79,8 @@ class Model:
         """Hand every part its tensors (names without the part's prefix).  Entries are
         removed from ``tensors`` as they are consumed so that fused copies do not double
         the memory for long."""
+        if self.fp8_weights:
+            raise ValueError("the model's weights are in 8 bits: load others into a new model")
         for spec, part in self._parts:
             names = type(part).param_specs(**spec.params)
             part.load({k: tensors.pop(spec.prefix + k) for k in names})
