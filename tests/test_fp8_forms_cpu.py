@@ -63,3 +63,19 @@ def test_other_weights_are_not_loaded_over_8_bit_ones(monkeypatch):
     model.use_fp8_weights()
     with pytest.raises(ValueError, match="8 bits"):
         model.load({})
+
+
+def test_pages_beside_which_one_layers_pages_fit_in_bfloat16():
+    """The pool of an 8-bit cache leaves room for the scratch of a step's portions: one layer's pages as bfloat16."""
+    from tiny_llm_infer_b200.cache import CacheManager
+    from tiny_llm_infer_b200.engine.llm_engine import estimate_num_kv_blocks
+    model = qwen()
+    model.use_fp8_cache(16)
+    needs, gib = model.cache_needs(), 1 << 30
+    eight = sum(CacheManager.bytes_per_page(needs, 16, torch.uint8).values())
+    mixer = model.blocks[0].mixer
+    layer = 2 * mixer.kv_heads * 16 * mixer.head_dim * 2
+    free, total = 40 * gib, 64 * gib
+    pages = estimate_num_kv_blocks(model, 16, torch.uint8, 256, 0.9, "cuda:0", memory=(free, total))
+    budget = int(total * 0.9) - (total - free) - total // 20
+    assert pages * (eight + layer) <= budget < (pages + 2) * (eight + layer + layer // 8)

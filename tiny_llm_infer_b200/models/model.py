@@ -103,6 +103,8 @@ class Model:
         for block in self.blocks:
             block.use_fp8_weights()
         self.fp8_weights = True
+        if torch.device(self.device).type == "cuda":
+            torch.cuda.empty_cache()        # what the bfloat16 matrices took: the cache's pool is sized from the device's free memory
 
     def use_fp8_cache(self, page_size: int) -> None:
         """Keep keys and values in 8 bits, from here on; cache managers for the model are then made with ``dtype=torch.uint8``.  A mixer
