@@ -76,3 +76,121 @@ def test_keys_of_missing_pages_do_not_count(n, gone, how):
     left = int(there.sum())
     want, off = exact_row(q[0].double().view(q_heads, dim), keys[:, there], values[:, there], left - 1, None, 1 / math.sqrt(dim))
     assert ((out[0].double() - want).abs() <= off).all()
+
+
+def dev(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def step_of(portions):
+    """A step of portions (slot, tokens, position of the first), as the runner lays them out: its context, positions and slots."""
+    from types import SimpleNamespace
+    seg, pos, slots, dec, tiles, row = [], [], [], [], [], 0
+    for s, (slot, n, first) in enumerate(portions):
+        seg.append((slot, row, n, first))
+        pos += range(first, first + n)
+        slots += [slot] * n
+        if n == 1:
+            dec.append(row)
+        else:
+            tiles += [(s, o) for o in range(0, n, 64)]
+        row += n
+    tiles.sort(key=lambda t: (t[1] % 256 != 0, t[1] % 128 != 0))
+    ctx = SimpleNamespace(tokens=row, segments=[SimpleNamespace(length=n, pos0=p) for _, n, p in portions], seg_info=dev(seg), dec_rows=dev(dec), n_dec=len(dec),
+                          pf_tiles=dev(tiles), n_tiles=len(tiles), n_tiles128=sum(t[1] % 128 == 0 for t in tiles), n_tiles256=sum(t[1] % 256 == 0 for t in tiles),
+                          max_context=max(first + n for _, n, first in portions))
+    return ctx, dev(pos), dev(slots)
+
+
+def check_portions(out, q, ctx, pos, slots, kept, q_heads, dim, window=None):
+    """Rows of portions: keys, values and the prompt kernels' weights pass through bfloat16 (2^-8 each) beside what a single token's do."""
+    single, scale = set(ctx.dec_rows.tolist()), 1 / math.sqrt(dim)
+    for i in range(ctx.tokens):
+        keys, values = kept[int(slots[i])]
+        p = int(pos[i])
+        want, off = exact_row(q[i].double().view(q_heads, dim), keys, values, p, window, scale)
+        if i not in single:
+            first = max(0, p + 1 - window) if window else 0
+            k, v = keys[:, first:p + 1], values[:, first:p + 1]
+            query = q[i].double().view(keys.shape[0], -1, dim)
+            e = (query.abs() @ k.abs().transpose(1, 2)).amax(-1, keepdim=True) * scale * 2.0 ** -8
+            mass = torch.softmax(query @ k.transpose(1, 2) * scale, dim=-1) @ v.abs()
+            off = off + (mass * (torch.expm1(2 * e) + 2 * 2.0 ** -8) * 1.02).reshape(-1)
+        assert ((out[i].double() - want).abs() <= off).all(), i
+
+
+def shared_prefix(g, requests, prefix, own, page, kv_heads, dim):
+    """Requests whose first ``prefix`` pages are the same ones, ``own`` further pages each, in a pool with room for one more."""
+    pages = prefix + requests * own + 1
+    planes = planes_of(pages, kv_heads, page, dim)
+    table = torch.empty((requests, prefix + own), dtype=torch.int32, device="cuda")
+    order = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+    table[:, :prefix] = order[:prefix]
+    table[:, prefix:] = order[prefix:prefix + requests * own].view(requests, own)
+    return planes, table
+
+
+def test_portions_that_share_a_prefix_take_no_more_than_the_pool():
+    """Five portions of 20 tokens behind 20 shared pages: scratch for the pool's 31 pages, not for the 110 that they list."""
+    from tiny_llm_infer_b200 import ops
+    g = gen(31)
+    q_heads, kv_heads, dim, page = 8, 8, 64, 64
+    planes, table = shared_prefix(g, 5, 20, 2, page, kv_heads, dim)
+    lengths = [20 * page + 20 + 12 * r for r in range(5)]
+    assert max(lengths) <= table.shape[1] * page
+    for r, n in enumerate(lengths):                             # the prefix is written once: the first request's
+        fill(g, planes, table[r:r + 1], [n], page, (0.3, 0.3))
+    ctx, pos, slots = step_of([(r, 20, n - 20) for r, n in enumerate(lengths)])
+    q = torch.randn((100, q_heads * dim), generator=g, device="cuda").to(torch.bfloat16)
+    out = torch.empty_like(q)
+
+    def call():
+        ops.paged_attention_fp8(q, planes, pos, slots, table, page, q_heads, kv_heads, dim, None, 1 / math.sqrt(dim), out, ctx)
+    call()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    call()
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - held <= planes[0].shape[0] * 2 * kv_heads * page * dim * 2 + (1 << 20)
+
+
+@pytest.mark.parametrize("dim,page,window", [(64, 32, None), (128, 16, None), (128, 48, 200)])
+def test_portions_that_share_pages(dim, page, window):
+    """Long shared prefixes, a single token beside them, and two portions whose tables are the same: one ends inside a page in which the
+    other goes on."""
+    from test_fp8_attention_gpu import stored
+    from tiny_llm_infer_b200 import ops
+    g = gen(dim + page)
+    q_heads, kv_heads, prefix = 8, 2, 9
+    planes, table = shared_prefix(g, 5, prefix, 3, page, kv_heads, dim)
+    table[4] = table[3]
+    start = prefix * page
+    new = [(0, 70, start - 40), (1, 33, start), (2, 1, start + 7), (3, 5, start + 1), (4, page, start + 6)]
+    lengths = [first + n for _, n, first in new]
+    assert max(lengths) <= table.shape[1] * page
+    for r in (0, 1, 2, 4):                                      # the fifth's table is the fourth's, and its tokens are more
+        fill(g, planes, table[r:r + 1], [lengths[r]], page, (0.3, 0.3))
+    ctx, pos, slots = step_of(new)
+    q = torch.randn((ctx.tokens, q_heads * dim), generator=g, device="cuda").to(torch.bfloat16)
+    out = torch.empty_like(q)
+    args = (planes, pos, slots, table, page, q_heads, kv_heads, dim, window, 1 / math.sqrt(dim))
+    ops.paged_attention_fp8(q, *args, out, ctx)
+    ops.check_error_word("cuda")
+    kept = [stored(planes, table, r, n, page) for r, n in enumerate(lengths)]
+    check_portions(out, q, ctx, pos, slots, kept, q_heads, dim, window)
+    # captured and replayed, for other portions of as many tokens
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.paged_attention_fp8(q, *args, out, ctx)
+    for back in (0, 3, 11):
+        other, p2, s2 = step_of([(r, n, first - back) for r, n, first in new])
+        other.max_context = ctx.max_context
+        ctx.seg_info.copy_(other.seg_info)
+        pos.copy_(p2)
+        out.fill_(7.0)
+        graph.replay()
+        want = torch.empty_like(q)
+        ops.paged_attention_fp8(q, planes, p2, s2, table, page, q_heads, kv_heads, dim, window, 1 / math.sqrt(dim), want, other)
+        assert torch.equal(out, want)
+    ops.check_error_word("cuda")

@@ -836,10 +836,14 @@ static int launch_attention_fp8(const A8Step& st, int blocks, int cluster, int* 
 // first key of its first token's window to the last token's, become pages of `pages` ([pages][keys, values][kv head][token][HD] bfloat16),
 // one portion after the other, and table[slot] lists them (-1 elsewhere).  The prompt kernels then read those.  One block of threads per
 // page; bound by HBM.
+// Portions that share pages (a common prefix) may list many times more than the cache has: then a page goes to the place of its own
+// number, `pages` as many as the cache's (kTails, kTokens).  Its tokens up to the last that any portion counts are written, all alike by
+// whichever portions list it; behind a portion's last token come zeros first, by a launch of their own, as another portion may go on there.
+enum A8Unpack : int { kInTurn = 0, kTails = 1, kTokens = 2 };
 template <int HD>
 __global__ void __launch_bounds__(256) attention_fp8_unpack_kernel(const A8Cache cache, const int* __restrict__ seg_info,
                                                                    const int* __restrict__ block_table, int max_pages, int page_size,
-                                                                   int kv_heads, int window, int capacity, bf16* __restrict__ pages,
+                                                                   int kv_heads, int window, int capacity, int places, bf16* __restrict__ pages,
                                                                    int* __restrict__ table) {
     TLLM_PDL_ENTER();
     const int seg = blockIdx.y;
@@ -851,13 +855,17 @@ __global__ void __launch_bounds__(256) attention_fp8_unpack_kernel(const A8Cache
         for (int n = threadIdx.x; n < max_pages; n += blockDim.x)
             if (n < first || n > last / page_size) table[(size_t)slot * max_pages + n] = -1;
     if (i > last / page_size || i >= max_pages) return;
-    int to = blockIdx.x;
-    for (int s = 0; s < seg; ++s)
-        if (seg_info[4 * s + 2] > 1 && seg_info[4 * s] >= 0)
-            to += (seg_info[4 * s + 3] + seg_info[4 * s + 2] - 1) / page_size - first_page(seg_info[4 * s + 3]) + 1;
-    const int page = to < capacity ? cache.held(block_table[(size_t)slot * max_pages + i]) : -1;
+    const int listed = cache.held(block_table[(size_t)slot * max_pages + i]);
+    int to = listed;
+    if (places == kInTurn) {
+        to = blockIdx.x;
+        for (int s = 0; s < seg; ++s)
+            if (seg_info[4 * s + 2] > 1 && seg_info[4 * s] >= 0)
+                to += (seg_info[4 * s + 3] + seg_info[4 * s + 2] - 1) / page_size - first_page(seg_info[4 * s + 3]) + 1;
+    }
+    const int page = to < capacity ? listed : -1;
     if (threadIdx.x == 0) table[(size_t)slot * max_pages + i] = page < 0 ? -1 : to;
-    if (page < 0) return;
+    if (page < 0 || (places == kTails && (i + 1) * page_size - 1 <= last)) return;
     const size_t at = (size_t)page * cache.stride, plane = (size_t)kv_heads * page_size;
     const float* scales = reinterpret_cast<const float*>(cache.scales + at);
     bf16* dst = pages + (size_t)to * 2 * plane * HD;
@@ -866,6 +874,7 @@ __global__ void __launch_bounds__(256) attention_fp8_unpack_kernel(const A8Cache
         const int token = n / kPer, which = token >= (int)plane, t = token - which * (int)plane;
         // tokens behind the last one hold what an earlier request left, or nothing: zeros instead
         const bool ok = i * page_size + t % page_size <= last;
+        if (places == (ok ? kTails : kTokens)) continue;
         const uint4 raw = ok ? *reinterpret_cast<const uint4*>((which ? cache.v : cache.k) + at + (size_t)t * HD + n % kPer * 16) : make_uint4(0, 0, 0, 0);
         const float s = ok ? scales[2 * t + which] : 0.0f;
         const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -936,20 +945,22 @@ extern "C" int tllm_attention_fp8_decode(const void* q, const void* k, const voi
 }
 
 // `held`: pages of the cache.  seg_info [segments][4] = slot, first row, tokens, position of the first.  `per`: pages of the portion that has most; pages bfloat16
-// [capacity][2][kv_heads][page_size][head_dim], room for all portions' pages; table int32 like block_table.
+// [capacity][2][kv_heads][page_size][head_dim], room for all portions' pages, or with `by_page` for as many as the cache has; table int32 like block_table.
 extern "C" int tllm_attention_fp8_unpack(const void* k, const void* v, const void* scales, long long page_bytes, int held, const int* seg_info, int segments,
                                          const int* block_table, int max_pages, int page_size, int kv_heads, int head_dim, int window, int per,
-                                         int capacity, void* pages, int* table, cudaStream_t stream) {
+                                         int capacity, int by_page, void* pages, int* table, cudaStream_t stream) {
     if (check_a8("attention_fp8_unpack", k, v, scales, page_bytes, held, page_size, kv_heads, head_dim) != 0) return -1;
     TLLM_REQUIRE(segments > 0 && segments <= 65535 && per > 0 && per <= max_pages && capacity > 0, "attention_fp8_unpack: bad sizes");
     TLLM_REQUIRE(seg_info && block_table && pages && table && (reinterpret_cast<uintptr_t>(pages) & 15u) == 0, "attention_fp8_unpack: missing operands");
-    TLLM_REQUIRE((long long)2 * kv_heads * page_size * (head_dim / 16) <= 0x7fffffff, "attention_fp8_unpack: too large");
+    TLLM_REQUIRE((long long)2 * kv_heads * page_size * (head_dim / 16) <= 0x7fffffff && (long long)max_pages * page_size <= 0x7fffffff, "attention_fp8_unpack: too large");
+    TLLM_REQUIRE(!by_page || capacity == held, "attention_fp8_unpack: %d places for the cache's %d pages", capacity, held);
     const A8Cache cache{(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)scales, page_bytes, held};
-    if (head_dim == 64)
-        launch_pdl(kPdlOther, attention_fp8_unpack_kernel<64>, dim3(per, segments), dim3(256), 0, stream, cache, seg_info, block_table, max_pages,
-                   page_size, kv_heads, window, capacity, (bf16*)pages, table);
-    else
-        launch_pdl(kPdlOther, attention_fp8_unpack_kernel<128>, dim3(per, segments), dim3(256), 0, stream, cache, seg_info, block_table, max_pages,
-                   page_size, kv_heads, window, capacity, (bf16*)pages, table);
-    return finish_launch("attention_fp8_unpack");
+    auto kernel = head_dim == 64 ? attention_fp8_unpack_kernel<64> : attention_fp8_unpack_kernel<128>;
+    for (int places = by_page ? kTails : kInTurn; places <= (by_page ? kTokens : kInTurn); ++places) {
+        launch_pdl(kPdlOther, kernel, dim3(per, segments), dim3(256), 0, stream, cache, seg_info, block_table, max_pages, page_size, kv_heads, window,
+                   capacity, places, (bf16*)pages, table);
+        const int rc = finish_launch("attention_fp8_unpack");
+        if (rc != 0) return rc;
+    }
+    return 0;
 }

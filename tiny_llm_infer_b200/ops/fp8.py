@@ -49,7 +49,7 @@ def declare(h) -> None:
         "tllm_qk_norm_rope_store_fp8": [vp, vp, vp, i32, f32, vp, i32, vp, vp, vp, i32, i32, vp, vp, vp, i64, i32, i32, vp, i32, i32, i32, i32,
                                         i32, vp, vp],
         "tllm_attention_fp8_decode": [vp, vp, vp, vp, i64, i32, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, f32, i32, i32, vp, vp, vp],
-        "tllm_attention_fp8_unpack": [vp, vp, vp, i64, i32, vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp],
+        "tllm_attention_fp8_unpack": [vp, vp, vp, i64, i32, vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp],
     }
     for name, args in sigs.items():
         fn = getattr(h, name)
@@ -502,7 +502,8 @@ def portion_pages(ctx, page_size: int, window: Optional[int], most: int, capturi
 
 def paged_attention_fp8(q, planes, positions, token_slot, block_table, page_size, q_heads, kv_heads, head_dim, window, scale, out, ctx=None):
     """``paged_attention`` over an 8-bit paged cache: one-token rows on ``paged_attention_decode_fp8``; the pages of longer segments are
-    brought back to bfloat16 in scratch, which the prompt kernels read.  Without a context every row is a one-token row."""
+    brought back to bfloat16 in scratch, at most as many as the cache has, which the prompt kernels read.  Without a context every row is a
+    one-token row."""
     ops = _ops()
     tokens = q.shape[0]
     if ctx is None or ctx.pf_tiles is None or ctx.tokens != tokens:
@@ -516,10 +517,12 @@ def paged_attention_fp8(q, planes, positions, token_slot, block_table, page_size
         k, v, s, stride, held = _planes(planes, page_size, kv_heads, head_dim)
         segments, most = ctx.seg_info.shape[0], min(-(-ctx.max_context // page_size), block_table.shape[1])
         per, capacity = portion_pages(ctx, page_size, window, most, torch.cuda.is_current_stream_capturing())
+        by_page = capacity > held                # portions that share pages: the places of the cache's own
+        capacity = min(capacity, held)
         pages = torch.empty((capacity, 2, kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=q.device)
         table = torch.empty_like(block_table)
         ops._check(ops.lib().tllm_attention_fp8_unpack(k, v, s, stride, held, ops._p(ctx.seg_info), segments, ops._p(block_table), block_table.shape[1], page_size,
-                                                       kv_heads, head_dim, int(window or 0), per, capacity, ops._p(pages), ops._p(table), ops._stream()),
-                   "attention_fp8_unpack")
+                                                       kv_heads, head_dim, int(window or 0), per, capacity, int(by_page), ops._p(pages), ops._p(table), ops._stream()),
+                   "attention_fp8_unpack", 2 if by_page else 1)
         ops._attention_tiles(q, pages, table, page_size, q_heads, kv_heads, head_dim, window, scale, out, ctx)
     return out
