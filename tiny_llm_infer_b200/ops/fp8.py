@@ -83,7 +83,7 @@ class Fp8Weight:
     """A weight [N, K] as e4m3 values ``q`` and float32 ``scales`` [ceil(N / 128), ceil(K / 128)].  ``gated``: the rows are N / 2 gate
     and N / 2 up rows interleaved by eight (``ops.interleave_gate_up``), and the scales [2 ceil(N / 2 / 128), ceil(K / 128)] are those
     of 128 gate rows, of the up rows that belong to them, and so on.  K is a multiple of 16."""
-    __slots__ = ("_q", "_scales", "gated", "shape", "device", "pointers", "index")
+    __slots__ = ("_q", "_scales", "gated", "shape", "device", "index", "_at")
 
     def __init__(self, q: torch.Tensor, scales: torch.Tensor, gated: bool = False):
         if q.dtype != E4M3 or q.dim() != 2 or scales.dtype != torch.float32:
@@ -99,9 +99,20 @@ class Fp8Weight:
         if q.device != scales.device or not q.is_contiguous() or not scales.is_contiguous() or q.data_ptr() % 16:
             _refuse("an 8-bit weight and its scales are contiguous on one device, the weight 16-byte aligned")
         self._q, self._scales, self.gated = q, scales, bool(gated)
-        # what every product asks for: the weight keeps its tensors, so their addresses are its own
+        # what every product asks for, of the tensors as they have been checked
         self.shape, self.device, self.index = q.shape, q.device, q.get_device()
-        self.pointers = (q.data_ptr(), scales.data_ptr())
+        self._at = (q.data_ptr(), scales.data_ptr())
+
+    def __reduce__(self):                        # a copy has places of its own
+        return Fp8Weight, (self._q, self._scales, self.gated)
+
+    @property
+    def pointers(self):
+        """Where values and scales lie."""
+        at = (self._q.data_ptr(), self._scales.data_ptr())
+        if at != self._at:
+            _refuse("the tensors of an 8-bit weight have been moved: make another weight of them")
+        return at
 
     @property
     def q(self) -> torch.Tensor:
@@ -130,7 +141,7 @@ class Fp8Weight:
 class Fp8Rows:
     """Rows [T, K] as e4m3 values ``q`` and float32 ``scales`` [T, ceil(K / 128)]: what the products take.  Rows that a kernel makes
     lie in one buffer, the values first; ``q`` and ``scales`` are views of it."""
-    __slots__ = ("shape", "pointers", "index", "_q", "_scales", "_buffer")
+    __slots__ = ("shape", "index", "_q", "_scales", "_buffer", "_at")
 
     def __init__(self, q: torch.Tensor, scales: torch.Tensor):
         if q.dtype != E4M3 or q.dim() != 2 or scales.dtype != torch.float32 or tuple(scales.shape) != (q.shape[0], _blocks(q.shape[1])):
@@ -141,7 +152,17 @@ class Fp8Rows:
         if q.device != scales.device or not q.is_contiguous() or not scales.is_contiguous() or q.data_ptr() % 16:
             _refuse("8-bit rows and their scales are contiguous on one device, the rows 16-byte aligned")
         self.shape, self._q, self._scales, self._buffer = q.shape, q, scales, None
-        self.pointers, self.index = (q.data_ptr(), scales.data_ptr()), q.get_device()
+        self._at, self.index = (q.data_ptr(), scales.data_ptr()), q.get_device()
+
+    def __reduce__(self):                        # a copy has places of its own
+        return Fp8Rows, (self.q, self.scales)
+
+    @property
+    def pointers(self):
+        """Where values and scales lie."""
+        if self._buffer is None and (self._q.data_ptr(), self._scales.data_ptr()) != self._at:
+            _refuse("the tensors of 8-bit rows have been moved: make other rows of them")
+        return self._at
 
     @property
     def q(self) -> torch.Tensor:
@@ -175,7 +196,7 @@ def _empty_rows(rows: int, k: int, device) -> Fp8Rows:
     made = Fp8Rows.__new__(Fp8Rows)              # right by construction
     made._buffer = buffer = torch.empty(rows * k + 4 * rows * -(-k // BLOCK), dtype=torch.uint8, device=device)
     at = buffer.data_ptr()
-    made.shape, made.pointers, made.index, made._q, made._scales = (rows, k), (at, at + rows * k), buffer.get_device(), None, None
+    made.shape, made._at, made.index, made._q, made._scales = (rows, k), (at, at + rows * k), buffer.get_device(), None, None
     return made
 
 
