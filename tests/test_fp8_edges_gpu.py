@@ -194,3 +194,26 @@ def test_portions_that_share_pages(dim, page, window):
         ops.paged_attention_fp8(q, planes, p2, s2, table, page, q_heads, kv_heads, dim, window, 1 / math.sqrt(dim), want, other)
         assert torch.equal(out, want)
     ops.check_error_word("cuda")
+
+
+def test_a_weight_made_of_rows_that_the_kernel_ahead_still_writes():
+    """The weight-streaming product fetches weights before the kernel ahead of it has ended.  Rows that have just been brought to 8 bits,
+    taken as a weight of one output, are there all the same."""
+    import fp8_reference as ref
+    from tiny_llm_infer_b200 import ops
+    g = gen(41)
+    k = 4096
+    x = torch.randn((4, k), generator=g, device="cuda").to(torch.bfloat16)
+    meet = ops.quantize_rows_fp8(x).values().double()
+    busy = torch.randn((4096, 4096), generator=g, device="cuda")
+    vectors = torch.randn((40, 1, k), generator=g, device="cuda").to(torch.bfloat16)
+    torch.cuda.synchronize()
+    kept = []
+    for v in vectors:
+        busy @ busy                                            # the host gets ahead: the kernels behind it start back to back
+        rows = ops.quantize_rows_fp8(v)
+        weight = ops.Fp8Weight(rows.q, rows.scales)
+        kept.append((rows, ops.linear(x, weight)))
+    for rows, y in kept:
+        exact, off = ref.product_bound(meet, rows.values().double(), torch.bfloat16)
+        assert ((y.double() - exact).abs() <= off).all()

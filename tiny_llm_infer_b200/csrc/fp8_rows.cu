@@ -140,8 +140,7 @@ add_rmsnorm_fp8_kernel(float* h, const TD* delta, const TG* __restrict__ gain, f
     }
 }
 
-// One block of 128 x 128 of a weight per thread block.  It lets no later kernel start early: the products fetch weights before they
-// wait for the kernel ahead of them.  GATED: q's rows are gate and up rows interleaved by eight (x has them so already); the
+// One block of 128 x 128 of a weight per thread block.  GATED: q's rows are gate and up rows interleaved by eight (x has them so already); the
 // scales' rows are a block of 128 gate rows, the block of their up rows, and so on.
 template <typename T>
 __global__ void __launch_bounds__(256) fp8_weight_kernel(const T* __restrict__ w, uint8_t* __restrict__ q, float* __restrict__ scales, int N,
@@ -178,6 +177,9 @@ __global__ void __launch_bounds__(256) fp8_weight_kernel(const T* __restrict__ w
     }
     if (threadIdx.x == 0) scales[(size_t)b * kb + blockIdx.x] = s;
 }
+
+// Nothing, by an ordinary launch: it starts when all before it in the stream has ended and is in memory, and lets nothing start early.
+__global__ void fp8_settle_kernel() {}
 
 template <typename TD, typename TG>
 static int launch_add_rmsnorm_fp8(float* h, const void* delta, const void* gain, float eps, void* q, float* scales, int rows, int width,
@@ -252,6 +254,13 @@ extern "C" int tllm_add_rmsnorm_fp8(float* h, const void* delta, int dtype, cons
                                    : launch_add_rmsnorm_fp8<bf16, float>(h, delta, gain, eps, q, scales, rows, width, stream);
     return gain_dtype == kBF16 ? launch_add_rmsnorm_fp8<float, bf16>(h, delta, gain, eps, q, scales, rows, width, stream)
                                : launch_add_rmsnorm_fp8<float, float>(h, delta, gain, eps, q, scales, rows, width, stream);
+}
+
+// Between what wrote a weight's tensors and its first product: the weight-streaming product fetches weights before the kernel ahead of it has
+// ended, and the kernels that make rows let it start at once.
+extern "C" int tllm_fp8_settle(cudaStream_t stream) {
+    fp8_settle_kernel<<<1, 32, 0, stream>>>();
+    return finish_launch("fp8_settle");
 }
 
 // w [N, K] (dtype) -> q [N, K] e4m3, scales [ceil(N / 128), ceil(K / 128)]; gated (N / 2 gate and N / 2 up rows interleaved by eight):

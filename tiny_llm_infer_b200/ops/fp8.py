@@ -46,6 +46,7 @@ def declare(h) -> None:
         "tllm_fp8_gated": [vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, f32, vp, vp, vp],
         "tllm_add_rmsnorm_fp8": [vp, vp, i32, vp, i32, f32, vp, vp, i32, i32, vp],
         "tllm_fp8_weight": [vp, i32, vp, vp, i32, i32, i32, vp],
+        "tllm_fp8_settle": [vp],
         "tllm_qk_norm_rope_store_fp8": [vp, vp, vp, i32, f32, vp, i32, vp, vp, vp, i32, i32, vp, vp, vp, i64, i32, i32, vp, i32, i32, i32, i32,
                                         i32, vp, vp],
         "tllm_attention_fp8_decode": [vp, vp, vp, vp, i64, i32, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, f32, i32, i32, vp, vp, vp],
@@ -82,7 +83,8 @@ def _here(*tensors) -> None:
 class Fp8Weight:
     """A weight [N, K] as e4m3 values ``q`` and float32 ``scales`` [ceil(N / 128), ceil(K / 128)].  ``gated``: the rows are N / 2 gate
     and N / 2 up rows interleaved by eight (``ops.interleave_gate_up``), and the scales [2 ceil(N / 2 / 128), ceil(K / 128)] are those
-    of 128 gate rows, of the up rows that belong to them, and so on.  K is a multiple of 16."""
+    of 128 gate rows, of the up rows that belong to them, and so on.  K is a multiple of 16.  Made on the stream that its tensors were
+    written on; a kernel of this package that writes them later is followed by some other work before the next product."""
     __slots__ = ("_q", "_scales", "gated", "shape", "device", "index", "_at")
 
     def __init__(self, q: torch.Tensor, scales: torch.Tensor, gated: bool = False):
@@ -102,6 +104,10 @@ class Fp8Weight:
         # what every product asks for, of the tensors as they have been checked
         self.shape, self.device, self.index = q.shape, q.device, q.get_device()
         self._at = (q.data_ptr(), scales.data_ptr())
+        if q.is_cuda:                            # products fetch weights before the kernel ahead of them has ended: what wrote these has
+            ops = _ops()
+            with torch.cuda.device(q.device):
+                ops._check(ops.lib().tllm_fp8_settle(ops._stream()), "fp8_settle")
 
     def __reduce__(self):                        # a copy has places of its own
         return Fp8Weight, (self._q, self._scales, self.gated)
