@@ -55,3 +55,10 @@ def test_rows_of_a_kernel_are_copied_with_their_buffer():
     other = copy.deepcopy(made)
     assert other.pointers == (other.q.data_ptr(), other.scales.data_ptr()) and other.pointers[0] != made.pointers[0]
     assert (other.q.view(torch.uint8) == 7).all() and (other.scales == 0.5).all()
+
+
+def test_8_bit_rows_take_an_8_bit_weight():
+    plain = torch.zeros((16, 144), dtype=torch.bfloat16)
+    for call in (ops.linear, ops.linear_swiglu):
+        with pytest.raises(ops.KernelError, match="8-bit weight"):
+            call(rows(), plain)

@@ -729,6 +729,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torch.dtyp
         if bias is not None:
             raise KernelError("a product with an 8-bit weight takes no bias")
         return linear_fp8(x, weight, out_dtype)
+    if isinstance(x, Fp8Rows):
+        raise KernelError("8-bit rows take an 8-bit weight")
     if not x.is_cuda:
         raise KernelError("linear takes CUDA tensors")
     want = out_dtype or x.dtype
