@@ -217,3 +217,127 @@ def test_a_weight_made_of_rows_that_the_kernel_ahead_still_writes():
     for rows, y in kept:
         exact, off = ref.product_bound(meet, rows.values().double(), torch.bfloat16)
         assert ((y.double() - exact).abs() <= off).all()
+
+
+@pytest.mark.parametrize("kv_heads,others,blocks", [(1, 0, 444), (8, 0, 444), (1, 59, 444), (1, 59, 100), (2, 29, 100)])
+def test_more_than_thirty_two_pieces(kv_heads, others, blocks):
+    """One long row in many pieces, alone (the warps of a block add them together) and beside short ones (a warp for a head), cut into
+    chunks and into equal shares."""
+    from tiny_llm_infer_b200 import ops
+    g = gen(kv_heads + others + blocks)
+    group, dim, page = 4, 128, 16
+    q_heads = kv_heads * group
+    lengths = [30001] + [1 + 7 * i % 90 for i in range(others)]
+    pages = sum(-(-n // page) for n in lengths) + 1
+    planes = planes_of(pages, kv_heads, page, dim)
+    table = tables(g, lengths, page, pages, -(-lengths[0] // page))
+    kept = fill(g, planes, table, lengths, page, (0.5, 1.0))
+    n = len(lengths)
+    q = (torch.randn((n, q_heads * dim), generator=g, device="cuda") * 2).to(torch.bfloat16)
+    pos, slots = dev([length - 1 for length in lengths]), dev(list(range(n)))
+    side, first = torch.cuda.Stream(), torch.full_like(q, 7.0)
+
+    def call(out):
+        return ops.paged_attention_decode_fp8(q, planes, pos, slots, None, n, table, page, q_heads, kv_heads, dim, None, 1 / math.sqrt(dim), out, lengths[0],
+                                              blocks=blocks)
+    call(first)
+    for r in range(n):
+        want, off = exact_row(q[r].double().view(q_heads, dim), *kept[r], lengths[r] - 1, None, 1 / math.sqrt(dim))
+        assert ((first[r].double() - want).abs() <= off).all()
+    # on another stream, and captured and replayed for other lengths
+    out = torch.full_like(q, 7.0)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(out)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    for back in (0, 1, 9000, 29990):
+        pos[0] = lengths[0] - 1 - back
+        graph.replay()
+        assert torch.equal(out, call(torch.full_like(q, 7.0)))
+        want, off = exact_row(q[0].double().view(q_heads, dim), *kept[0], lengths[0] - 1 - back, None, 1 / math.sqrt(dim))
+        assert ((out[0].double() - want).abs() <= off).all()
+
+
+@pytest.mark.parametrize("what", ["query nan", "query inf", "key nan", "value nan", "key scale nan", "key scale inf", "value scale nan", "value scale inf"])
+@pytest.mark.parametrize("how", WAYS)
+def test_numbers_that_are_none(what, how):
+    """They reach what the formula gives them to and nothing else: the other heads, the other dims of a value."""
+    g = gen(len(what))
+    page, kv_heads, q_heads, dim, n, key = 16, 2, 8, 128, 300, 217
+    planes, table, (keys, values), at, place = a_request(g, n, page, kv_heads, dim)
+    scales = planes[2].view(torch.float32)
+    q = torch.randn((1, q_heads * dim), generator=g, device="cuda").to(torch.bfloat16)
+    keys, values = keys.clone(), values.clone()
+    odd = float("nan") if what.endswith("nan") else float("inf")
+    if what.startswith("query"):
+        q[0, dim + 5] = odd                                    # head 1
+    elif what == "key nan":
+        planes[0][at[key], 1, place[key], 9] = 0x7F
+        keys[1, key, 9] = odd
+    elif what == "value nan":
+        planes[1][at[key], 1, place[key], 9] = 0x7F
+        values[1, key, 9] = odd
+    else:
+        which = 0 if what.startswith("key") else 1
+        old = scales[at[key], 1, place[key], which].double()
+        scales[at[key], 1, place[key], which] = odd
+        if which:
+            values[1, key] = values[1, key] / old * odd
+    out = attend(q, planes, n, table, page, q_heads, kv_heads, dim, **how)[0].double()
+    query = q[0].double().view(kv_heads, -1, dim)
+    s = query @ keys.transpose(1, 2) / math.sqrt(dim)
+    if what.startswith("key scale"):                           # a score is its product times the scale
+        s[1, :, key] = s[1, :, key] * odd
+    p = torch.softmax(s, dim=-1)
+    want = (p @ values).reshape(-1)
+    finite = torch.isfinite(want)
+    # where the formula has no number there is none; an infinite scale of a value is one of all its dims
+    assert not torch.isfinite(out[~finite]).any() and (~finite).any() and finite.any()
+    assert torch.isfinite(out[finite]).all()
+    clean = torch.nan_to_num(keys, 0.0, 0.0, 0.0), torch.nan_to_num(values, 0.0, 0.0, 0.0)
+    if what != "key scale inf":                                # there the other keys of a head share its weight
+        _, off = exact_row(torch.nan_to_num(query, 0.0, 0.0, 0.0).reshape(q_heads, dim), *clean, n - 1, None, 1 / math.sqrt(dim))
+        assert ((out - want).abs() <= off)[finite].all()
+
+
+@pytest.mark.parametrize("t,n,k", [(2048, 6144, 4096), (1000, 10240, 2064), (1500, 4112, 12288)])
+def test_products_by_pairs_that_turn_their_rings(t, n, k):
+    """Tens of blocks of K a tile and several tiles a pair of SMs: every stage is used many times over."""
+    import fp8_reference as ref
+    from test_fp8_products_gpu import rows_of
+    from tiny_llm_infer_b200 import ops
+    assert ops.fp8._plan(t, n, k, 148)[0] == ops.fp8.PAIRS
+    g = gen(t + n)
+    x, w = rows_of(g, t, k, torch.bfloat16), rows_of(g, n, k, torch.float32) * 0.02
+    weight, rows = ops.quantize_weight_fp8(w), ops.quantize_rows_fp8(x)
+    y = ops.linear(x, weight)
+    ops.check_error_word("cuda")
+    exact, off = ref.product_bound(rows.values().double(), weight.values().double(), torch.bfloat16)
+    assert ((y.double() - exact).abs() <= off).all()
+    assert torch.equal(y, ops.linear(rows, weight))
+
+
+@pytest.mark.parametrize("t,inter,k", [(600, 12288, 4096), (2048, 2064, 2064)])
+def test_gated_products_by_pairs_that_turn_their_rings(t, inter, k):
+    import fp8_reference as ref
+    from tiny_llm_infer_b200 import ops
+    assert ops.fp8._plan(t, 2 * inter, k, 148, gated=True)[0] == ops.fp8.PAIRS
+    g = gen(t + inter)
+    x = (torch.randn((t, k), generator=g, device="cuda") * 2).to(torch.bfloat16)
+    gate, up = (torch.randn((inter, k), generator=g, device="cuda") * 0.02 for _ in range(2))
+    weight, rows = ops.quantize_weight_fp8(ops.interleave_gate_up(gate, up), gated=True), ops.quantize_rows_fp8(x)
+    got = ops.linear_swiglu(x, weight)
+    ops.check_error_word("cuda")
+    values = weight.values().double().view(inter // 8, 2, 8, k)
+    (zg, dg), (zu, du) = (ref.product_bound(rows.values().double(), values[:, i].reshape(inter, k), torch.float32) for i in (0, 1))
+    a = zg * torch.sigmoid(zg)
+    exact = a * zu
+    off = 1.2 * dg * zu.abs() + du * a.abs() + 1.2 * dg * du + 2.0 ** -19 * zg.abs() * zu.abs()      # the slope of silu is at most 1.1
+    per = got.scales[:, ref.block_of(inter, "cuda")]
+    assert ((got.values().double() - exact).abs() <= off + ref.half_step(exact.abs() + off, per)).all()
+    assert (got.scales <= ref.row_scales((exact.abs() + off).float()) * (1 + 2.0 ** -20)).all()
+    assert (got.scales >= ref.row_scales((exact.abs() - off).clamp_min(0).float()) * (1 - 2.0 ** -20)).all()
