@@ -79,3 +79,24 @@ def test_pages_beside_which_one_layers_pages_fit_in_bfloat16():
     pages = estimate_num_kv_blocks(model, 16, torch.uint8, 256, 0.9, "cuda:0", memory=(free, total))
     budget = int(total * 0.9) - (total - free) - total // 20
     assert pages * (eight + layer) <= budget < (pages + 2) * (eight + layer + layer // 8)
+
+
+@pytest.mark.parametrize("form", ["weights", "cache"])
+def test_a_runner_is_of_the_form_that_its_model_had(form, monkeypatch):
+    """Its graphs hold the places of the matrices and pages that they were captured with."""
+    from tiny_llm_infer_b200.cache import CacheManager
+    from tiny_llm_infer_b200.engine import ModelRunner, StepEntry
+    from tiny_llm_infer_b200.engine.runner import StepError
+    monkeypatch.setattr(ops, "quantize_weight_fp8", lambda w, gated=False: None)
+    model = qwen()
+    for block in model.blocks:
+        block.ffn.inter = 352
+    cache = CacheManager(model.cache_needs(), 16, 8, max_slots=2, max_seq_len=64, dtype=torch.bfloat16, device="cpu")
+    runner = ModelRunner(model, cache, max_batch_tokens=64)
+    prepared = runner.prepare([StepEntry("a", [1, 2, 3], [2])])
+    monkeypatch.setattr(model, "forward", lambda *a: pytest.fail("the step was run"))
+    model.use_fp8_weights() if form == "weights" else model.use_fp8_cache(16)
+    with pytest.raises(StepError, match="form"):
+        runner.run(prepared)
+    with pytest.raises(StepError, match="form"):
+        runner.step([StepEntry("a", [1, 2, 3], [2])])

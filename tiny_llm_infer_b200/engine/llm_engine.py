@@ -300,7 +300,8 @@ class LLM:
     ``quantization`` "fp8": the layers' matrices are kept in 8 bits (e4m3, a float32 scale per block of 128 x 128) and meet rows rounded
     to 8 bits per 128 columns; embedding, norms and head stay in bfloat16.  ``kv_cache_dtype`` "fp8": keys and values are kept in
     8 bits, a float32 scale per token and head, half the memory and half the reading.  Both are for bfloat16 models of the
-    architectures whose parts have the form (Qwen3); others are refused.  A model given as ``loaded`` keeps the form from then on.
+    architectures whose parts have the form (Qwen3); others are refused.  A model given as ``loaded`` keeps the form from then on,
+    and engines made of it before refuse their next step.
     """
 
     def __init__(self, model: str, dtype: str = "bfloat16", max_model_len: int = 2048,

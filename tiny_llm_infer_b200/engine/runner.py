@@ -101,6 +101,7 @@ class ModelRunner:
     def __init__(self, model: Model, cache: CacheManager, max_batch_tokens: int = 8192,
                  use_graphs: bool = True, prompt_graphs: bool = False):
         self.model, self.cache = model, cache
+        self._form = model.form                    # graphs hold the places of the matrices and pages of this form
         self.use_graphs = use_graphs
         self.prompt_graphs = prompt_graphs and use_graphs
         self._graphs = {}
@@ -137,6 +138,10 @@ class ModelRunner:
         self._dev = torch.empty(12 * n + 64, dtype=torch.int32, device=self.device)
         self._uploaded: Optional[torch.cuda.Event] = None
         self._prepared: Optional[PreparedStep] = None      # the host buffer holds this step
+
+    def _check_form(self) -> None:
+        if self.model.form != self._form:
+            raise StepError("the model's weights or cache have taken another form (8 bits) since this runner was made: make a new one")
 
     def check_kernels(self, step: Optional[PreparedStep] = None) -> None:
         """Raise if a kernel with bounded waits gave up since the last check (reads a device
@@ -267,6 +272,7 @@ class ModelRunner:
             raise StepError("a prepared step has not been run yet")
         if not entries:
             raise StepError("a step needs at least one entry")
+        self._check_form()
         if self.use_graphs and self._graphable(entries):
             prepared = self._prepare_graph(entries)
         elif self.use_graphs and self._rows_graphable(entries):
@@ -288,6 +294,7 @@ class ModelRunner:
         if prepared is not self._prepared:
             raise StepError("run() takes the step that prepare() returned last")
         self._prepared = None                      # whatever happens below, the host buffer is free again
+        self._check_form()
         host = self._host.numpy()
         n_late, words = len(prepared.late), prepared.upload
         if late_source is not None:

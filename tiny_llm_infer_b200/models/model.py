@@ -89,6 +89,11 @@ class Model:
         self.loaded = True
 
     # ---- 8 bits
+    @property
+    def form(self) -> Tuple[bool, bool]:
+        """Whether weights and cache are in 8 bits.  A runner is of the form that its model had when it was made."""
+        return self.fp8_weights, self.fp8_cache
+
     def use_fp8_weights(self) -> None:
         """Keep the matrices of every block in 8 bits (once, after ``load``).  Embedding, norms and head stay as they are.  A block or
         a part without that form is refused before any has changed its own."""
