@@ -341,3 +341,50 @@ def test_gated_products_by_pairs_that_turn_their_rings(t, inter, k):
     assert ((got.values().double() - exact).abs() <= off + ref.half_step(exact.abs() + off, per)).all()
     assert (got.scales <= ref.row_scales((exact.abs() + off).float()) * (1 + 2.0 ** -20)).all()
     assert (got.scales >= ref.row_scales((exact.abs() - off).clamp_min(0).float()) * (1 - 2.0 ** -20)).all()
+
+
+def test_calls_of_no_rows():
+    """A step's part without rows is an empty result, as with the bfloat16 operators, not an error."""
+    from tiny_llm_infer_b200 import ops
+    width, inter, q_heads, kv_heads, dim, page = 64, 32, 4, 2, 64, 16
+    weight = ops.quantize_weight_fp8(torch.randn((48, width), device="cuda"))
+    gated = ops.quantize_weight_fp8(torch.randn((2 * inter, width), device="cuda"), gated=True)
+    h = torch.zeros((0, width), device="cuda")
+    rows = ops.add_rmsnorm_fp8(h, None, torch.ones(width, device="cuda"), 1e-6)
+    for x in (h, h.to(torch.bfloat16), rows, ops.quantize_rows_fp8(h)):
+        assert tuple(ops.linear(x, weight).shape) == (0, 48)
+        got = ops.linear_swiglu(x, gated)
+        assert tuple(got.shape) == tuple(got.q.shape) == (0, inter) and tuple(got.scales.shape) == (0, 1) and tuple(got.values().shape) == (0, inter)
+    planes = planes_of(3, kv_heads, page, dim)
+    before = [p.clone() for p in planes]
+    table, none = torch.zeros((1, 3), dtype=torch.int32, device="cuda"), dev([])
+    q = torch.zeros((0, q_heads * dim), dtype=torch.bfloat16, device="cuda")
+    qkv = torch.zeros((0, (q_heads + 2 * kv_heads) * dim), dtype=torch.bfloat16, device="cuda")
+    ops.qk_norm_rope_store_fp8(qkv, None, None, 1.0, None, 0, none, none, table, planes, page, torch.empty_like(q), q_heads, kv_heads, dim,
+                               ops.QK_STORE | ops.QK_QOUT)
+    assert all(torch.equal(a, b) for a, b in zip(planes, before))
+    ops.paged_attention_decode_fp8(q, planes, none, none, None, 0, table, page, q_heads, kv_heads, dim, None, 0.1, torch.empty_like(q), 48)
+    ops.paged_attention_fp8(q, planes, none, none, table, page, q_heads, kv_heads, dim, None, 0.1, torch.empty_like(q))
+    # rows there, none of them asked for
+    q, one = torch.zeros((2, q_heads * dim), dtype=torch.bfloat16, device="cuda"), dev([0, 0])
+    out = torch.full_like(q, 7.0)
+    ops.paged_attention_decode_fp8(q, planes, one, one, none, 0, table, page, q_heads, kv_heads, dim, None, 0.1, out, 48)
+    assert (out == 7).all()
+
+
+@pytest.mark.parametrize("t,n,k", [(70001, 264, 144), (65536, 136, 272)])
+def test_products_of_very_many_rows(t, n, k):
+    import fp8_reference as ref
+    from tiny_llm_infer_b200 import ops
+    g = gen(t)
+    x = torch.randn((t, k), generator=g, device="cuda").to(torch.bfloat16)
+    w = torch.randn((n // 16 * 16, k), generator=g, device="cuda") * 0.1
+    weight, gated, rows = ops.quantize_weight_fp8(w), ops.quantize_weight_fp8(w[:128].contiguous(), gated=True), ops.quantize_rows_fp8(x)
+    exact, off = ref.product_bound(rows.values().double(), weight.values().double(), torch.bfloat16)
+    assert ((ops.linear(x, weight).double() - exact).abs() <= off).all()
+    few = ops.linear_swiglu(ops.Fp8Rows(rows.q[-7:].contiguous(), rows.scales[-7:].contiguous()), gated)
+    many = ops.linear_swiglu(x, gated)
+    ops.check_error_word("cuda")
+    # the last rows by another kernel: within the rounding to 8 bits of each
+    a, b, scale = few.values(), many.values()[-7:], torch.maximum(few.scales, many.scales[-7:])
+    assert ((a - b).abs() <= torch.maximum(a.abs(), b.abs()) * 2.0 ** -3 * 1.01 + scale * 2.0 ** -9).all()

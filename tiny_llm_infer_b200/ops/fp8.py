@@ -444,6 +444,8 @@ def qk_norm_rope_store_fp8(qkv: torch.Tensor, q_gain, k_gain, eps: float, inv_fr
     if q_out is not None and (q_out.dtype != torch.bfloat16 or tuple(q_out.shape) != (tokens, q_heads * head_dim)):
         _refuse(f"qk_norm_rope_store_fp8: queries go to bfloat16 [{tokens}, {q_heads * head_dim}], got {q_out.dtype} {tuple(q_out.shape)}")
     k, v, s, stride, held = _planes(planes, page_size, kv_heads, head_dim) if planes is not None else (None, None, None, 0, 0)
+    if tokens == 0:
+        return
     ops._check(ops.lib().tllm_qk_norm_rope_store_fp8(
         ops._p(qkv), ops._p(q_gain), ops._p(k_gain), ops._dt(q_gain) if q_gain is not None else ops.F32, float(eps), ops._p(inv_freq), rotary_dim,
         ops._p(positions), ops._p(token_slot), ops._p(block_table),
@@ -500,6 +502,8 @@ def paged_attention_decode_fp8(q, planes, positions, token_slot, rows, n_rows, b
     _attention_operands("paged_attention_decode_fp8", q, out, positions, token_slot, rows, n_rows, block_table, q_heads, kv_heads, head_dim)
     k, v, s, stride, held = _planes(planes, page_size, kv_heads, head_dim)
     max_pages = block_table.shape[1]
+    if n_rows == 0:
+        return out
     if blocks is None and cluster is None:
         reach = min(max_context, max_pages * page_size)
         blocks, cluster = attention_cut(n_rows, kv_heads, q_heads // kv_heads, min(reach, window) if window else reach, ops.SM_COUNT)
