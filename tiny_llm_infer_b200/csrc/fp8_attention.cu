@@ -463,8 +463,8 @@ __device__ __forceinline__ A8Row row_at(const A8Step& st, int r, int slot, int g
 // A block of threads per (row, key/value head), the whole of it one run.  No kernel that follows may start before this one ends (and the same for clusters
 // below): bfloat16 products that start early hold their places and fetch beside it (eight layers of Qwen3-8B widths, 8 rows of 4096 keys: 1.39 ms
 // a step where it takes 0.89; one row 1.00 and 0.73).  ORDERED, for more blocks than are resident at once: the rows with most
-// keys first, so that what starts late is short (64 rows of 800 to 4096 keys, 8 heads of
-// 128: 56 us where equal shares took 64; sizes all alike are the one case that shares do better, 117 and 98).
+// keys first, so that what starts late is short (64 rows of 1024 to 4096 keys, 8 heads of
+// 128: 62 us where equal shares take 72; 64 rows all of 4096, which shares do better, 119 and 99).
 constexpr int kA8MaxOrdered = 256;
 template <int HD, int NT, bool ORDERED>
 __global__ void __launch_bounds__(kA8Warps * 32, NT == 1 ? 3 : 2) attention_fp8_whole_kernel(const A8Step st, bf16* __restrict__ out) {
@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(kA8Warps * 32, NT == 1 ? 3 : 2) attention_fp8_
 
 // Longer ones of few rows: a cluster of `size` blocks per (row, key/value head), each with an equal run of its keys, whose sums are added in
 // the order of the keys through distributed shared memory.  One kernel, no scratch, and no plan to be made before the first key is fetched.
-// (One row of 4095 keys for 32 heads on 8: 10.7 us, in shares 13.2, a block per head 34; 8 rows of up to 4096: 17 to 18, 20 to 23 and 34.)
+// (One row of 4095 keys for 32 heads on 8: 10.7 us, in shares 13.1, a block per head 34; 8 rows of up to 4096: 17 to 18, 20 to 23 and 34.)
 constexpr int kA8MaxCluster = 8;
 __device__ __forceinline__ float peer_float(uint32_t address, int rank) {
     float v;

@@ -1,6 +1,6 @@
 """Weights, rows and caches in 8 bits: e4m3 values with float32 scales, and the kernels that read them (``csrc/fp8*.cu``).
 
-A block of numbers with largest magnitude A is kept as e4m3(x / s) and s = max(A, 2^-100) / 448.  A weight has a scale per
+A block of numbers with largest magnitude A is kept as e4m3(x (1 / s)) and s = max(A, 2^-100) / 448, in float32.  A weight has a scale per
 block of 128 x 128, a row that meets it one per 128 columns, a key or value of the cache one per head.  A product sums the 128 terms of
 a block in float32, multiplies by both scales and adds the blocks in float32:
 
@@ -470,11 +470,15 @@ SHARED_ROWS = 512        # rows that may share blocks
 def attention_cut(rows: int, kv_heads: int, group: int, reach: int, sms: int):
     """(blocks that share all rows' keys, blocks of a cluster) for ``paged_attention_decode_fp8``: (0, 1) for one block per (row, key/value head),
     (0, 2 to 8) for a cluster of them, (as many as are resident, 1) for shares and a second kernel that adds them; whichever should take least,
-    in us, for rows of at most ``reach`` keys, 0.65 of them on average.  A block of its own: 4.1, and 0.9 for every 128 keys, up to 1.4 times that where
+    in us, for rows of at most ``reach`` keys.  The lengths are on the device: rows are taken to hold 0.65 of the longest on average, and heads to be 128 wide.
+    A block of its own: 4.1, and 0.9 for every 128 keys, up to 1.4 times that where
     SMs have several, or what HBM takes for all keys.  A cluster: 5.4, 1 for every 100 blocks, and 0.95 to 1.3 for every 128 keys of a block.  Shares: 12, and 2.4
-    for every 32 keys that a warp gets.  (Measured, us, own block, cluster, shares, rows x heads of 128, longest: 1 x 8, 1000 12.2, 6.7, 10.0; 1 x 8, 4095
-    34, 10.7, 13.2; 1 x 8, 16384 117, 21.4, 18.7; 8 x 8, 1000 12.9, 10.3, 14.7; 8 x 8, 4095 34, 16.7, 20.1; 16 x 8, 4095 34, 25.9, 27.4; 24 x 8, 4096 41, 34, 35;
-    37 x 8, 4096 43, 54, 49; 64 x 8, 4096 56, -, 64, all equally long 117 and 98; 128 x 8, 4096 123, -, 129.)"""
+    for every 32 keys that a warp gets.
+    Measured, us, own block, best cluster, shares, rows x heads of 128, rows between a quarter of the longest and all of it: 1 x 8, 1000 11.3, 6.7, 10.1;
+    1 x 8, 4095 34, 10.7, 13.1; 1 x 8, 16384 117, 21.6, 18.6; 8 x 8, 1000 12.9, 10.4, 14.5; 8 x 8, 4095 34, 17.4, 19.8; 16 x 8, 4095 34, 26.7, 26.8; 24 x 8, 4096 43,
+    35, 35; 37 x 8, 4096 47, -, 49; 64 x 8, 4096 62, -, 72; 128 x 8, 4096 122, -, 125; 64 x 8 of 64, 4096 40, -, 48.
+    Rows all of one length, for which the rule is not always right: 8 x 8, 4095 34, 18.4, 23; 16 x 8, 4095 35, 29, 34 (it takes shares);
+    24 x 8, 4096 45, 41, 46; 37 x 8, 4096 53, -, 61; 64 x 8, 4096 119, -, 99 (a block each, in two waves); 128 x 8, 4096 187, -, 182; 64 x 8 of 64, 4096 68, -, 58."""
     if rows == 0:
         return 0, 1
     pairs, mean = rows * kv_heads, 0.65 + 0.35 / rows
@@ -533,8 +537,9 @@ def portion_pages(ctx, page_size: int, window: Optional[int], most: int, capturi
 
 def paged_attention_fp8(q, planes, positions, token_slot, block_table, page_size, q_heads, kv_heads, head_dim, window, scale, out, ctx=None):
     """``paged_attention`` over an 8-bit paged cache: one-token rows on ``paged_attention_decode_fp8``; the pages of longer segments are
-    brought back to bfloat16 in scratch, at most as many as the cache has, which the prompt kernels read.  Without a context every row is a
-    one-token row."""
+    brought back to bfloat16 in scratch, at most as many as the cache has, which the prompt kernels read: there a key or value is rounded once more,
+    after its scale.  Every page that a portion sees is held, as ``paged_attention`` has it: the prompt kernels read a missing one as zeros, where one-token
+    rows leave its keys out.  Without a context every row is a one-token row."""
     ops = _ops()
     tokens = q.shape[0]
     if ctx is None or ctx.pf_tiles is None or ctx.tokens != tokens:
