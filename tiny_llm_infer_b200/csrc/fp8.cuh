@@ -2,12 +2,12 @@
 // mma.sync.
 //
 // A block of numbers (128 neighbours of a row, 128 x 128 of a weight, one head of a key or value) with largest magnitude A is kept as
-// q = e4m3(x (1 / s)), s = max(A, 2^-100) / 448, both quotients and the product rounded to float32: the largest becomes
-// +-448, the largest e4m3 value, a rounding is off by at most 2^-4 of the number down to 2^-6 s (the smallest normal e4m3) and by 2^-10 s below,
-// give or take 2^-22 of the number: where x / s lies that near to the middle of two e4m3 values, either may be taken.  (A division per number
-// in place of the product: 2048 x 12288 rows 21.1 us for 14.5, eight rows by 6144 x 4096 13.4 for 9.0; the product and its remainder added back, which
-// gives the rounded quotient, 16.1 and 9.6.)  The floor under A keeps s and 1 / s normal, so a block of zeros becomes zeros.  An infinity makes the block's s infinite and itself NaN, a NaN becomes NaN: the
-// sums that meet them are NaN.
+// q = e4m3(x (1 / s)), s = max(A, 2^-100) / 448, both quotients and the product rounded to float32: the largest becomes +-448, the
+// largest e4m3 value, a rounding is off by at most 2^-4 of the number down to 2^-6 s (the smallest normal e4m3) and by 2^-10 s below,
+// give or take 2^-22 of the number: where x / s lies that near to the middle of two e4m3 values, either may be taken.  (A division per
+// number in place of the product: 2048 x 12288 rows 21.1 us for 14.5, eight rows by 6144 x 4096 13.4 for 9.0; the product and its
+// remainder added back, which gives the rounded quotient, 16.1 and 9.6.)  The floor under A keeps s and 1 / s normal, so a block of
+// zeros becomes zeros.  An infinity makes the block's s infinite and itself NaN, a NaN becomes NaN: the sums that meet them are NaN.
 #pragma once
 
 #include <cuda_fp16.h>
